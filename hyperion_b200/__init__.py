@@ -116,6 +116,8 @@ EXT_FUNCTIONS = [
     "hyb_kv_copy_layer", "hyb_kv_cursor", "hyb_prefill_logits", "hyb_decode_logits", "hyb_decode_forced",
     "hyb_test_arm_post_append_fault", "hyb_model_set_memory_budget", "hyb_sample_logits",
     "hyb_model_weight_bytes", "hyb_qmv_unpack", "hyb_embed_packed",
+    "hyb_paged_plan", "hyb_qkv_post_paged", "hyb_sdpa_shared_prefix_scratch_bytes", "hyb_sdpa_shared_prefix",
+    "hyb_sample_batch",
 ]
 
 _lib: Optional[ctypes.CDLL] = None
@@ -184,6 +186,14 @@ def lib() -> ctypes.CDLL:
         "hyb_test_arm_post_append_fault": [],
         "hyb_model_set_memory_budget": [P, c.c_uint64],
         "hyb_model_weight_bytes": [P, c.POINTER(c.c_uint64), c.POINTER(c.c_uint64), c.POINTER(c.c_uint64)],
+        "hyb_paged_plan": [P, P, c.c_int32, c.c_int32, c.c_int32, P, c.c_int32, P, c.c_int32, c.c_int32, c.c_int32,
+                           P, P, P, P, P, P, P],
+        "hyb_qkv_post_paged": [P, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, P, P, P, P, P,
+                               c.c_int32, c.c_float, P, P, P, P],
+        "hyb_sdpa_shared_prefix": [P, P, P, c.c_int32, c.c_int32, P, c.c_int32, P, c.c_int32, P, P, P, c.c_int32,
+                                   c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32,
+                                   c.c_float, c.c_float, P, P, c.c_size_t, P],
+        "hyb_sample_batch": [P, c.c_int32, c.c_int32, c.c_int32, c.c_int64, P, P, P, P, P, P, P, P, P],
         "hyb_sample_logits": [P, c.c_int32, ctypes.POINTER(HypSamplingConfig), c.c_uint64, P, P],
     }
     for name, args in sig.items():
@@ -192,6 +202,8 @@ def lib() -> ctypes.CDLL:
         fn.restype = S
     L.hyb_sdpa_decode_scratch_bytes.argtypes = [c.c_int32, c.c_int32, c.c_int32, c.c_int32]
     L.hyb_sdpa_decode_scratch_bytes.restype = c.c_size_t
+    L.hyb_sdpa_shared_prefix_scratch_bytes.argtypes = [c.c_int32] * 8
+    L.hyb_sdpa_shared_prefix_scratch_bytes.restype = c.c_size_t
     L.hyb_qmv_packed_bytes.argtypes = [c.c_int64, c.c_int64]
     L.hyb_qmv_packed_bytes.restype = c.c_size_t
     _lib = L

@@ -310,4 +310,88 @@ void launch_prefill_attn_tc(const PrefillAttnParams& p, cudaStream_t stream);
 void launch_prefill_attn_mma(const PrefillAttnParams& p, cudaStream_t stream);
 int64_t read_attn_tc_wait_timeouts();
 
+// ---------------------------------------------------------------- paged batch decode
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device (asked once).
+void allow_smem(const void* kernel, size_t bytes);
+
+// Block tables, slot map and row tables of a batch from its requests' lengths (paged.cu).
+constexpr int kMaxPlanRequests = 8192;
+struct PagedPlanParams {
+    const int* cached = nullptr;      // [n_req] tokens already in the cache
+    const int* added = nullptr;       // [n_req] tokens this step adds
+    int n_req = 0, page_size = 0, n_pages = 0;
+    const int* free_pages = nullptr;  // [n_free]
+    int n_free = 0;
+    int* table = nullptr;             // [n_req][max_blocks], extended in place
+    int max_blocks = 0, pos0 = 0, max_rows = 0;
+    int* row_start = nullptr;         // [n_req + 1]
+    int* row_req = nullptr;           // [max_rows], -1 behind the last row
+    int* row_pos = nullptr;
+    int* slot_map = nullptr;
+    int* total_lens = nullptr;        // [n_req]
+    int* status = nullptr;            // pages taken, rows, requests refused, bad pages
+};
+void launch_paged_plan(const PagedPlanParams& p, cudaStream_t stream);
+
+// QK-norm + RoPE + cache write through a slot map (paged.cu).
+struct QkvPostPagedParams {
+    const bf16* qkv = nullptr;        // [T][ld]: q | k | v, or q | k with v_from_k
+    int T = 0, ld = 0, n_heads = 0, n_kv = 0, hd = 0;
+    bool v_from_k = false;
+    const bf16* q_norm = nullptr;
+    const bf16* k_norm = nullptr;
+    const float* inv_freq = nullptr;  // [hd / 2]
+    const int* row_pos = nullptr;     // [T], < 0: a padding row
+    const int* slot_map = nullptr;    // [T], outside [0, n_slots): not cached
+    int n_slots = 0;
+    float eps = 1e-6f;
+    bf16* q_out = nullptr;            // [T][n_heads][hd]
+    bf16* k_pool = nullptr;           // [n_slots][n_kv][hd]
+    bf16* v_pool = nullptr;
+};
+void launch_qkv_post_paged(const QkvPostPagedParams& p, cudaStream_t stream);
+
+// Attention of a batch's rows over one shared prefix and each request's own pages
+// (attention_paged.cu).
+struct SharedAttnParams {
+    const bf16* q = nullptr;           // [T][n_heads][hd]
+    const bf16* k_pool = nullptr;      // [n_pages][page_size][n_kv][hd]
+    const bf16* v_pool = nullptr;
+    int n_pages = 0, page_size = 0;
+    const int* prefix_table = nullptr; // [ceil(prefix_len / page_size)]
+    int prefix_len = 0;
+    const int* table = nullptr;        // [n_req][max_blocks]
+    int max_blocks = 0;
+    const int* own_lens = nullptr;     // [n_req]
+    const int* row_start = nullptr;    // [n_req + 1]
+    const int* row_pos = nullptr;      // [T]
+    int T = 0, n_req = 0, max_q = 0, max_own = 0;
+    int n_heads = 0, n_kv = 0, hd = 0, window = 0;
+    float scale = 1.f, softcap = 0.f;
+    bf16* out = nullptr;               // [T][n_heads][hd]
+    void* scratch = nullptr;
+    size_t scratch_bytes = 0;
+};
+size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
+                                 int hd);
+void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream);
+
+// Batched sampling of [rows][ld] logits from given uniforms (sampler_batch.cu).
+constexpr int kMaxSampleVocab = 1 << 19;
+struct SampleBatchParams {
+    const void* logits = nullptr;
+    bool f32 = false;                 // float logits, else bf16
+    int rows = 0, vocab = 0;
+    int64_t ld = 0;                   // elements between rows
+    const float* u = nullptr;         // [rows]
+    const float* temperature = nullptr;  // [rows] or null (1.0)
+    const int* top_k = nullptr;          // [rows] or null (off)
+    const float* top_p = nullptr;
+    const float* min_p = nullptr;
+    int* token = nullptr;             // [rows]
+    int* kept = nullptr;              // [rows] or null
+    float* prob = nullptr;            // [rows] or null
+};
+void launch_sample_batch(const SampleBatchParams& p, cudaStream_t stream);
+
 }  // namespace hyb

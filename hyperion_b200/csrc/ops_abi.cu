@@ -3,6 +3,7 @@
 #include "hyperion_b200.h"
 #include "kernels.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstddef>
 #include <cstdio>
@@ -394,6 +395,170 @@ HypStatus hyb_qkv_post(const void* qkv, int32_t L, int32_t ld, int32_t n_heads, 
         p.cache_cap = cache_cap;
         p.cache_first = cache_first;
         hyb::launch_qkv_post(p, as_stream(stream));
+    });
+}
+
+HypStatus hyb_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int32_t n_req, int32_t page_size,
+                         int32_t n_pages, const int32_t* free_pages, int32_t n_free, int32_t* block_table,
+                         int32_t max_blocks, int32_t pos0, int32_t max_rows, int32_t* row_start, int32_t* row_req,
+                         int32_t* row_pos, int32_t* slot_map, int32_t* total_lens, int32_t* status, void* stream) {
+    if (!cached_lens || !new_lens || !block_table || !row_start || !row_req || !row_pos || !slot_map || !total_lens || !status)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "null pointer argument");
+    if (n_free < 0 || (n_free > 0 && !free_pages)) return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: bad free list");
+    if (n_req < 1 || n_req > hyb::kMaxPlanRequests) return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: n_req must be 1..8192");
+    if (page_size < 1 || n_pages < 1 || max_blocks < 1 || max_rows < 1 || pos0 < 0)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: bad shape");
+    if (static_cast<int64_t>(n_pages) * page_size > INT32_MAX || static_cast<int64_t>(max_blocks) * page_size + pos0 > INT32_MAX)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: slots and positions must stay below 2^31");
+    return run([&] {
+        hyb::PagedPlanParams p;
+        p.cached = cached_lens;
+        p.added = new_lens;
+        p.n_req = n_req;
+        p.page_size = page_size;
+        p.n_pages = n_pages;
+        p.free_pages = free_pages;
+        p.n_free = n_free;
+        p.table = block_table;
+        p.max_blocks = max_blocks;
+        p.pos0 = pos0;
+        p.max_rows = max_rows;
+        p.row_start = row_start;
+        p.row_req = row_req;
+        p.row_pos = row_pos;
+        p.slot_map = slot_map;
+        p.total_lens = total_lens;
+        p.status = status;
+        hyb::launch_paged_plan(p, as_stream(stream));
+    });
+}
+
+HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                             int32_t v_from_k, const void* q_norm, const void* k_norm, const float* inv_freq,
+                             const int32_t* row_pos, const int32_t* slot_map, int32_t n_slots, float eps, void* q_out,
+                             void* k_pool, void* v_pool, void* stream) {
+    if (!qkv || !q_norm || !k_norm || !inv_freq || !row_pos || !slot_map || !q_out || !k_pool || !v_pool)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "null pointer argument");
+    if (T < 1 || n_heads < 1 || n_kv < 1 || n_slots < 1) return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "qkv_post_paged: bad shape");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return hyb::abi_fail(HYP_STATUS_UNSUPPORTED, "qkv_post_paged: head_dim must be 64, 128 or 256");
+    const int64_t need = (static_cast<int64_t>(n_heads) + (v_from_k ? 1 : 2) * static_cast<int64_t>(n_kv)) * head_dim;
+    if (ld < need) return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "qkv_post_paged: ld smaller than the q/k/v columns");
+    if (ld % 8 != 0 || !aligned16(qkv) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(q_out) ||
+        !aligned16(k_pool) || !aligned16(v_pool))
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "qkv_post_paged: rows must start on 16-byte boundaries");
+    return run([&] {
+        hyb::QkvPostPagedParams p;
+        p.qkv = static_cast<const hyb::bf16*>(qkv);
+        p.T = T;
+        p.ld = ld;
+        p.n_heads = n_heads;
+        p.n_kv = n_kv;
+        p.hd = head_dim;
+        p.v_from_k = v_from_k != 0;
+        p.q_norm = static_cast<const hyb::bf16*>(q_norm);
+        p.k_norm = static_cast<const hyb::bf16*>(k_norm);
+        p.inv_freq = inv_freq;
+        p.row_pos = row_pos;
+        p.slot_map = slot_map;
+        p.n_slots = n_slots;
+        p.eps = eps;
+        p.q_out = static_cast<hyb::bf16*>(q_out);
+        p.k_pool = static_cast<hyb::bf16*>(k_pool);
+        p.v_pool = static_cast<hyb::bf16*>(v_pool);
+        hyb::launch_qkv_post_paged(p, as_stream(stream));
+    });
+}
+
+static bool shared_shape_ok(int32_t T, int32_t n_req, int32_t max_q, int32_t max_own, int32_t prefix_len,
+                            int32_t n_heads, int32_t n_kv) {
+    return T >= 1 && n_req >= 1 && max_q >= 1 && max_own >= 0 && prefix_len >= 0 && n_kv >= 1 && n_heads >= 1 &&
+           n_heads % n_kv == 0 && n_heads <= 65536 && static_cast<int64_t>(prefix_len) + max_own <= INT32_MAX - 65536;
+}
+
+size_t hyb_sdpa_shared_prefix_scratch_bytes(int32_t T, int32_t n_req, int32_t max_q, int32_t max_own,
+                                            int32_t prefix_len, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+    if (!shared_shape_ok(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv) ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        return 0;
+    return hyb::shared_attn_scratch_bytes(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, head_dim);
+}
+
+HypStatus hyb_sdpa_shared_prefix(const void* q, const void* k_pool, const void* v_pool, int32_t n_pages,
+                                 int32_t page_size, const int32_t* prefix_table, int32_t prefix_len,
+                                 const int32_t* block_table, int32_t max_blocks, const int32_t* own_lens,
+                                 const int32_t* row_start, const int32_t* row_pos, int32_t T, int32_t n_req,
+                                 int32_t max_q, int32_t max_own, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                 int32_t window, float scale, float softcap, void* out, void* scratch,
+                                 size_t scratch_bytes, void* stream) {
+    if (!q || !k_pool || !v_pool || !block_table || !own_lens || !row_start || !row_pos || !out || !scratch ||
+        (prefix_len > 0 && !prefix_table))
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "null pointer argument");
+    if (!shared_shape_ok(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv) || n_pages < 1 || max_blocks < 1 || window < 0)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sdpa_shared_prefix: bad shape");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return hyb::abi_fail(HYP_STATUS_UNSUPPORTED, "sdpa_shared_prefix: head_dim must be 64, 128 or 256");
+    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+        return hyb::abi_fail(HYP_STATUS_UNSUPPORTED, "sdpa_shared_prefix: page_size must be 16, 32, 64, 128 or 256");
+    if (static_cast<int64_t>(n_pages) * page_size > INT32_MAX)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sdpa_shared_prefix: the pool's slots must stay below 2^31");
+    if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || !aligned16(scratch))
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sdpa_shared_prefix: q, pools, out and scratch must be 16-byte aligned");
+    return run([&] {
+        hyb::SharedAttnParams p;
+        p.q = static_cast<const hyb::bf16*>(q);
+        p.k_pool = static_cast<const hyb::bf16*>(k_pool);
+        p.v_pool = static_cast<const hyb::bf16*>(v_pool);
+        p.n_pages = n_pages;
+        p.page_size = page_size;
+        p.prefix_table = prefix_table;
+        p.prefix_len = prefix_len;
+        p.table = block_table;
+        p.max_blocks = max_blocks;
+        p.own_lens = own_lens;
+        p.row_start = row_start;
+        p.row_pos = row_pos;
+        p.T = T;
+        p.n_req = n_req;
+        p.max_q = std::min(max_q, T);
+        p.max_own = max_own;
+        p.n_heads = n_heads;
+        p.n_kv = n_kv;
+        p.hd = head_dim;
+        p.window = window;
+        p.scale = scale;
+        p.softcap = softcap;
+        p.out = static_cast<hyb::bf16*>(out);
+        p.scratch = scratch;
+        p.scratch_bytes = scratch_bytes;
+        hyb::launch_shared_attn(p, as_stream(stream));
+    });
+}
+
+HypStatus hyb_sample_batch(const void* logits, int32_t f32, int32_t rows, int32_t vocab, int64_t ld, const float* u,
+                           const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                           int32_t* token, int32_t* kept, float* prob, void* stream) {
+    if (!logits || !u || !token) return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "null pointer argument");
+    if (rows < 1 || rows > (1 << 20) || vocab < 1 || vocab > hyb::kMaxSampleVocab || ld < vocab)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sample_batch: bad shape (1..2^20 rows of 1..2^19 logits)");
+    if (reinterpret_cast<uintptr_t>(logits) % (f32 ? 4 : 2) != 0)
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sample_batch: logits are not aligned to their type");
+    return run([&] {
+        hyb::SampleBatchParams p;
+        p.logits = logits;
+        p.f32 = f32 != 0;
+        p.rows = rows;
+        p.vocab = vocab;
+        p.ld = ld;
+        p.u = u;
+        p.temperature = temperature;
+        p.top_k = top_k;
+        p.top_p = top_p;
+        p.min_p = min_p;
+        p.token = token;
+        p.kept = kept;
+        p.prob = prob;
+        hyb::launch_sample_batch(p, as_stream(stream));
     });
 }
 

@@ -226,6 +226,109 @@ HypStatus hyb_sample_logits(const void* logits, int32_t n, const HypSamplingConf
                             void* result, void* stream);
 
 /*
+ * ---- Batch decode over a paged KV cache (no reference counterpart: the reference keeps one
+ * contiguous cache per sequence). A pool is bf16 [n_pages, page_size, n_kv, head_dim]; token
+ * j of a request lives in slot block_table[j / page_size] * page_size + j % page_size. The
+ * four calls below are one serving step: hyb_paged_plan, then per layer hyb_qkv_post_paged
+ * and hyb_sdpa_shared_prefix, then hyb_sample_batch. None allocates device memory, reads
+ * back or synchronises, so a step can be captured into a graph and replayed while the
+ * lengths on the device change. Device pointers belong to the current device.
+ */
+
+/*
+ * Block tables, slot map and row tables of a batch, from its requests' lengths (all int32
+ * on the device). Request b holds cached_lens[b] tokens and adds new_lens[b] (0 is fine).
+ *   row_start [n_req + 1]: exclusive prefix sums of the new tokens; rows beyond max_rows are
+ *   cut off. For row r of request b, the i-th of its new ones: row_req[r] = b, row_pos[r] =
+ *   pos0 + cached + i (pos0: the length of a prefix kept elsewhere), slot_map[r] = its slot.
+ *   All three [max_rows] arrays are -1 behind the last row.
+ *   block_table [n_req, max_blocks], in place: the ceil((cached + new) / page_size) -
+ *   ceil(cached / page_size) pages that request b needs are taken from free_pages [n_free]
+ *   in request order; other entries are neither changed nor, but for the page that a
+ *   request's new tokens continue, read. The same lengths give the same result again: the
+ *   free list is not changed, and the caller drops its first status[0] entries.
+ *   total_lens [n_req]: tokens after the step, cached + new.
+ *   status [4]: pages taken, rows, requests refused, and pages outside [0, n_pages) among
+ *   those taken or continued (rows on them get slot -1). A request is refused when a length is
+ *   negative, its tokens do not fit max_blocks, its rows do not fit max_rows, or the free list
+ *   is used up: it takes no page, total_lens stays cached (0 if that is negative), and its rows
+ *   (none if a length is negative) get slot -1. A later request that needs no page still runs.
+ * n_req is 1..8192; n_pages * page_size and pos0 + max_blocks * page_size are below 2^31.
+ */
+HypStatus hyb_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int32_t n_req, int32_t page_size,
+                         int32_t n_pages, const int32_t* free_pages, int32_t n_free, int32_t* block_table,
+                         int32_t max_blocks, int32_t pos0, int32_t max_rows, int32_t* row_start, int32_t* row_req,
+                         int32_t* row_pos, int32_t* slot_map, int32_t* total_lens, int32_t* status, void* stream);
+
+/*
+ * hyb_qkv_post for rows of many requests: QK-norm, RoPE at row_pos[t] and the cache write to
+ * slot_map[t] of the pools (n_slots = n_pages * page_size). qkv: bf16 [T, ld] as there. In
+ * contrast to it everything is computed in fp32 and rounded to bf16 once, and the angle
+ * row_pos * inv_freq is reduced in double, so that far positions keep their accuracy.
+ * A row with row_pos < 0 is skipped (its q_out row stays as it was); one whose slot lies
+ * outside the pools gets q_out but writes no cache. The slots of one call must be distinct.
+ * head_dim 64, 128 or 256; ld a multiple of 8; pointers but the int32 and float ones 16-byte
+ * aligned. qkv must not overlap the outputs.
+ */
+HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                             int32_t v_from_k, const void* q_norm, const void* k_norm, const float* inv_freq,
+                             const int32_t* row_pos, const int32_t* slot_map, int32_t n_slots, float eps, void* q_out,
+                             void* k_pool, void* v_pool, void* stream);
+
+/*
+ * Attention of a batch whose requests share a prefix: the prefix's keys and values are read
+ * once for all rows, each request's own pages once for its rows, and the parts are joined.
+ *   q, out: bf16 [T, n_heads, head_dim]. Request b's rows are row_start[b] .. row_start[b+1]
+ *   (one each for a decode step, 2..9 for speculative verify, more for a prefill chunk).
+ *   Key positions: prefix key j (prefix_table [ceil(prefix_len / page_size)]) is at j, request
+ *   b's own key j < own_lens[b] (block_table [n_req, max_blocks]) at prefix_len + j. Row t
+ *   sees the keys at positions <= row_pos[t] and, with window > 0, > row_pos[t] - window.
+ *   scale and softcap as in hyb_sdpa_decode; scores, statistics and sums are fp32, the
+ *   unnormalised probabilities are rounded to bf16.
+ *   A row that sees no key gets zeros. Rows of no request (before row_start[0] or from
+ *   row_start[n_req] on) and rows with row_pos < 0 stay as they were.
+ *   max_q and max_own are host bounds on a request's rows and own keys: they size the launch
+ *   and the scratch (hyb_sdpa_shared_prefix_scratch_bytes with the same values; contents do
+ *   not matter before or after). Rows at or past max_q of a request, and rows of a request
+ *   with more than max_own or max_blocks * page_size keys, become NaN; so do rows some of
+ *   whose tile of rows read a page outside [0, n_pages). A negative own_lens counts as 0.
+ *   Slots that no row of the call sees may hold anything (NaN included); the ones that some
+ *   row sees must be finite.
+ * head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; n_pages * page_size < 2^31;
+ * q, the pools, out and scratch 16-byte aligned.
+ */
+size_t hyb_sdpa_shared_prefix_scratch_bytes(int32_t T, int32_t n_req, int32_t max_q, int32_t max_own,
+                                            int32_t prefix_len, int32_t n_heads, int32_t n_kv, int32_t head_dim);
+HypStatus hyb_sdpa_shared_prefix(const void* q, const void* k_pool, const void* v_pool, int32_t n_pages,
+                                 int32_t page_size, const int32_t* prefix_table, int32_t prefix_len,
+                                 const int32_t* block_table, int32_t max_blocks, const int32_t* own_lens,
+                                 const int32_t* row_start, const int32_t* row_pos, int32_t T, int32_t n_req,
+                                 int32_t max_q, int32_t max_own, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                 int32_t window, float scale, float softcap, void* out, void* scratch,
+                                 size_t scratch_bytes, void* stream);
+
+/*
+ * Sampling of a batch of logit rows with settings per row, from given uniforms (in place of
+ * hyb_sample_logits' generator): logits bf16 (f32 = 0) or float (f32 = 1) [rows, ld], of
+ * which vocab (1..2^19) count. Per row, from device arrays [rows] (a null array: the
+ * default): temperature (1), top_k (off at <= 0 or >= vocab), top_p (off unless in (0, 1)),
+ * min_p (off unless > 0), and u in [0, 1).
+ *   Weights are w = exp((x - max x) / temperature), tokens ordered by logit descending, then
+ *   index ascending. Each filter keeps a prefix of that order: the first top_k; the shortest
+ *   whose weight reaches top_p of the whole row's; those with w >= min_p. The shortest of the
+ *   three is kept, and token is the first index, in index order, at which the running sum
+ *   of the kept weights exceeds u times their sum. temperature <= 0 (or NaN) takes the
+ *   first maximum. kept (may be null) is the number of tokens kept, prob (may be null) the
+ *   drawn token's share of the kept weight. NaN logits count as -inf; a row without any
+ *   logit above -inf gives token -1, kept 0, prob 0; +inf logits share all the weight.
+ *   u outside [0, 1) is clamped. Sums are exact integers: results do not depend on the
+ *   batch, the order of additions or the run.
+ */
+HypStatus hyb_sample_batch(const void* logits, int32_t f32, int32_t rows, int32_t vocab, int64_t ld, const float* u,
+                           const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                           int32_t* token, int32_t* kept, float* prob, void* stream);
+
+/*
  * RMSNorm over rows of length D: out = bf16(bf16(x * rsqrt(mean(x^2) + eps)) * w);
  * w may be NULL (the weightless v_norm). Replaces mx::fast::rms_norm
  * (native/hyperion_mlx/src/forward.cc:25-27).

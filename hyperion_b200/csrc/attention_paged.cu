@@ -14,7 +14,7 @@
 // Statistics and accumulators are fp32. The probabilities are rounded to bf16 for the
 // tensor cores, as unnormalised exp(s - m) <= 1, and l sums the rounded ones, so that the
 // rounding cancels where all weights round alike.
-#include "kernels.h"
+#include "attention_paged.cuh"
 #include "tma.cuh"
 
 #include <algorithm>
@@ -24,13 +24,6 @@ namespace hyb {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
@@ -53,15 +46,6 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// How a call's keys are split (the same on the host for the scratch size, the grid and the
-// merge).
-struct SharedPlan {
-    int tiles_p = 0, split_p = 0;  // 16-row tiles over all rows; parts of the prefix
-    int tiles_o = 0, split_o = 0;  // 16-row tiles of one request; parts of its own keys
-    int chunk_o = 0;               // own keys of one part
-    __host__ __device__ int splits() const { return split_p + split_o; }
-};
-
 constexpr int kTileRows = 16;
 constexpr int kWarps = 4;
 constexpr int kSlice = 16;             // keys of one warp step
@@ -71,13 +55,29 @@ SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len,
     SharedPlan s;
     const int G = n_heads / n_kv;
     max_q = std::min(max_q, T);
-    s.tiles_p = static_cast<int>((static_cast<long long>(T) * G + kTileRows - 1) / kTileRows);
-    s.tiles_o = static_cast<int>((static_cast<long long>(max_q) * G + kTileRows - 1) / kTileRows);
-    if (prefix_len > 0) {
+    const long long all_rows = static_cast<long long>(T) * G, req_rows = static_cast<long long>(max_q) * G;
+    auto tiles = [](long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); };
+    // Tiles of one request's rows when they fill 128-row tiles about as well as the whole
+    // batch's rows do: then prefix and own keys are one pass.
+    const bool per_request = req_rows > kTileRows && 4ll * n_req * tiles(req_rows, kTcRows) <= 5ll * tiles(all_rows, kTcRows);
+    if (per_request) {
+        s.tc_per_request = 1;
+        s.tc_tiles = tiles(req_rows, kTcRows);
+    } else if (prefix_len > 0 && all_rows > kTileRows) {
+        s.tc_tiles = tiles(all_rows, kTcRows);
+    }
+    if (s.tc_tiles > 0) {
+        const long long units = static_cast<long long>(s.tc_tiles) * n_kv * (per_request ? n_req : 1);
+        const long long blocks = (prefix_len + (per_request ? max_own : 0) + 63) / 64;
+        s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((blocks + 1) / 2, 148 / units)));
+        if (per_request) return s;
+    } else if (prefix_len > 0) {
+        s.tiles_p = tiles(all_rows, kTileRows);
         const long long units = static_cast<long long>(s.tiles_p) * n_kv;
         s.split_p = static_cast<int>(std::max<long long>(1, std::min<long long>((prefix_len + 63) / 64, kTargetCtas / units)));
     }
     if (max_own > 0) {
+        s.tiles_o = tiles(req_rows, kTileRows);
         const long long units = static_cast<long long>(s.tiles_o) * n_kv * n_req;
         const long long want = std::max<long long>(1, std::min<long long>((max_own + 63) / 64, 2 * kTargetCtas / units));
         s.chunk_o = static_cast<int>(((max_own + want - 1) / want + 63) / 64 * 64);
@@ -85,12 +85,6 @@ SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len,
     }
     return s;
 }
-
-// Scratch: fp32 partial outputs [T][n_heads][splits][hd], then (m, l) pairs [T][n_heads][splits].
-struct Parts {
-    float* o;
-    float2* ml;
-};
 
 template <int HD>
 struct SmallPlan {
@@ -111,7 +105,7 @@ struct SmallPlan {
 // traffic as one: HBM bound.
 template <int HD>
 __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const SharedAttnParams p, const SharedPlan pl,
-                                                                        Parts parts) {
+                                                                        SharedParts parts) {
     using SP = SmallPlan<HD>;
     constexpr int KS = HD / 16, CH = HD / 8;
     extern __shared__ __align__(128) unsigned char sm[];
@@ -234,7 +228,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
     };
 #pragma unroll
     for (int i = 0; i < SP::kStages - 1; ++i) fetch(i);
-    const float scale2 = p.scale * kLog2e;
+    const float scale2 = p.scale * kSharedLog2e;
     for (int i = 0; i < mine; ++i) {
         fetch(i + SP::kStages - 1);
         cp_wait<SP::kStages - 1>();
@@ -254,7 +248,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
             }
         }
         auto shape = [&](float dot, int key, int pos) {
-            float s = p.softcap > 0.f ? p.softcap * kLog2e * tanhf(dot * p.scale / p.softcap) : dot * scale2;
+            float s = p.softcap > 0.f ? p.softcap * kSharedLog2e * tanhf(dot * p.scale / p.softcap) : dot * scale2;
             const int kp = base + key;
             const bool see = key >= lo && key < hi && kp <= pos && (p.window == 0 || kp > pos - p.window);
             return see ? s : -INFINITY;
@@ -277,7 +271,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
         // a row that has seen no key keeps m = -inf; 0 stands in so that no inf - inf appears
         const float zA = nA == -INFINITY ? 0.f : nA, zB = nB == -INFINITY ? 0.f : nB;
         if (__any_sync(0xffffffffu, nA != mA || nB != mB)) {
-            const float aA = ex2(mA - zA), aB = ex2(mB - zB);
+            const float aA = shared_ex2(mA - zA), aB = shared_ex2(mB - zB);
             lA *= aA;
             lB *= aB;
 #pragma unroll
@@ -294,7 +288,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float z = j < 2 ? zA : zB;
-            pf[j] = pack_bf2(f2bf(ex2(v[2 * j] - z)), f2bf(ex2(v[2 * j + 1] - z)));
+            pf[j] = pack_bf2(f2bf(shared_ex2(v[2 * j] - z)), f2bf(shared_ex2(v[2 * j + 1] - z)));
             const float sum = __uint_as_float(pf[j] << 16) + __uint_as_float(pf[j] & 0xffff0000u);
             if (j < 2) lA += sum;
             else lB += sum;
@@ -336,7 +330,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
         *reinterpret_cast<float2*>(so + (g + 8) * HD + 8 * d + c2) = make_float2(o[d][2], o[d][3]);
     }
     __syncthreads();
-    const int at = prefix ? split : pl.split_p + split;
+    const int at = pl.tc_splits + (prefix ? split : pl.split_p + split);
     for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += kWarps * 32) {
         const int m = idx / (HD / 4), d = 4 * (idx % (HD / 4));
         float M = -INFINITY;
@@ -347,7 +341,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = ex2(s_m[w][m] - z);
+            const float f = shared_ex2(s_m[w][m] - z);
             const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm) + (w * kTileRows + m) * HD + d);
             L += f * s_l[w][m];
             acc.x += f * x.x;
@@ -357,8 +351,8 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
         }
         const long long pr = m0 + m;
         const size_t row = static_cast<size_t>(t0 + pr / G) * p.n_heads + hk * G + pr % G;
-        *reinterpret_cast<float4*>(parts.o + (row * pl.splits() + at) * HD + d) = acc;
-        if (d == 0) parts.ml[row * pl.splits() + at] = make_float2(M, L);
+        if (L != 0.f) *reinterpret_cast<float4*>(parts.o + (row * parts.n + at) * HD + d) = acc;
+        if (d == 0) parts.ml[row * parts.n + at] = make_float2(M, L);
     }
 }
 
@@ -367,7 +361,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
 // breaks the bounds the caller gave (more rows than max_q, more keys than max_own or its
 // table) has parts that were not computed and becomes NaN.
 template <int HD>
-__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParams p, int splits, Parts parts) {
+__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParams p, SharedParts parts) {
     const int lane = threadIdx.x & 31;
     const long long unit = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     if (unit >= static_cast<long long>(p.T) * p.n_heads) return;
@@ -382,6 +376,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParam
     const int own = p.own_lens[lo];
     const bool broken = t - p.row_start[lo] >= p.max_q || own > p.max_own ||
                         own > static_cast<long long>(p.max_blocks) * p.page_size;
+    const int splits = parts.n;
     const float2* ml = parts.ml + unit * splits;
     const float* src = parts.o + unit * splits * HD;
     float M = -INFINITY;
@@ -395,7 +390,8 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParam
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
     for (int s = 0; s < splits; ++s) {
         const float2 v = ml[s];
-        const float f = ex2(v.x - z);
+        if (v.y == 0.f) continue;  // no key of the part is seen
+        const float f = shared_ex2(v.x - z);
         L += f * v.y;
 #pragma unroll
         for (int i = 0; i < PER; ++i) acc[i] += f * src[static_cast<size_t>(s) * HD + lane * PER + i];
@@ -411,10 +407,11 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParam
 }
 
 template <int HD>
-void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, Parts parts, cudaStream_t stream) {
+void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, SharedParts parts, cudaStream_t stream) {
     using SP = SmallPlan<HD>;
     const long long n_prefix = static_cast<long long>(pl.tiles_p) * p.n_kv * pl.split_p;
     const long long n_own = static_cast<long long>(pl.tiles_o) * p.n_kv * pl.split_o * p.n_req;
+    if (pl.tc_splits > 0) launch_shared_attn_tc(p, pl, parts, stream);
     if (n_prefix + n_own > INT_MAX) throw ArgError("sdpa_shared_prefix: too many parts");
     if (n_prefix + n_own > 0) {
         allow_smem(reinterpret_cast<const void*>(shared_attn_small_kernel<HD>), SP::kSmem);
@@ -422,7 +419,7 @@ void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, Parts part
         HYB_LAUNCH_CHECK("shared_attn_small_kernel");
     }
     const long long warps = static_cast<long long>(p.T) * p.n_heads;
-    shared_merge_kernel<HD><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(p, pl.splits(), parts);
+    shared_merge_kernel<HD><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(p, parts);
     HYB_LAUNCH_CHECK("shared_merge_kernel");
 }
 
@@ -440,9 +437,10 @@ void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
     const size_t units = static_cast<size_t>(p.T) * p.n_heads * pl.splits();
     if (p.scratch_bytes < shared_attn_scratch_bytes(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd))
         throw ArgError("sdpa_shared_prefix: scratch too small");
-    Parts parts;
+    SharedParts parts;
     parts.o = static_cast<float*>(p.scratch);
     parts.ml = reinterpret_cast<float2*>(parts.o + units * p.hd);
+    parts.n = pl.splits();
     switch (p.hd) {
         case 64: launch_shared_t<64>(p, pl, parts, stream); break;
         case 128: launch_shared_t<128>(p, pl, parts, stream); break;

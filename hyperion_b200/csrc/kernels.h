@@ -375,6 +375,7 @@ struct SharedAttnParams {
 size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
                                  int hd);
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream);
+int64_t read_shared_attn_wait_timeouts();
 
 // Batched sampling of [rows][ld] logits from given uniforms (sampler_batch.cu).
 constexpr int kMaxSampleVocab = 1 << 19;

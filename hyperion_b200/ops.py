@@ -160,44 +160,52 @@ def qkv_post(qkv, n_heads, n_kv, hd, v_from_k, q_norm, k_norm, inv_freq, pos0, e
 
 
 # ---------------------------------------------------------------- batch decode over a paged cache
-def _on(ref: torch.Tensor, **tensors):
-    """Checks of the paged ops' arguments: every given tensor (value: tensor, dtype, shape or
-    None) sits on `ref`'s CUDA device, has its dtype and shape and is contiguous."""
-    if not ref.is_cuda:
+# A decode step calls these every few microseconds of GPU work, so the checks are written for the
+# host's time: one comparison chain per tensor, plain integers for the C arguments, and a stream
+# or device switch only where the call asks for one.
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+
+
+def _bad(name, t, dtype, shape, dev):
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def _ck(name, t, dtype, shape, dev):
+    """The pointer of a contiguous tensor of this type, shape and device."""
+    if t.get_device() != dev or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _bad(name, t, dtype, shape, dev)
+    return t.data_ptr()
+
+
+def _ck_opt(name, t, dtype, shape, dev):
+    return None if t is None else _ck(name, t, dtype, shape, dev)
+
+
+def _device(t):
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("the paged ops take CUDA tensors")
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None:
-            continue
-        if t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
-        if t.dtype != dtype:
-            raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+    return dev
 
 
-class _Launch:
-    """The device and the stream of a call: `stream` or the device's current one, made current
-    so that what the call allocates belongs to that stream."""
-
-    def __init__(self, device, stream):
-        self.stream = stream if stream is not None else torch.cuda.current_stream(device)
-        if self.stream.device != device:
-            raise ValueError(f"the stream is on {self.stream.device}, the tensors on {device}")
-        self.ctx = torch.cuda.stream(self.stream)
-
-    def __enter__(self):
-        self.ctx.__enter__()
-        return ctypes.c_void_p(self.stream.cuda_stream)
-
-    def __exit__(self, *exc):
-        self.ctx.__exit__(*exc)
+def _switch(dev, stream):
+    """None where the call can go to the current stream as it is; otherwise the context that makes
+    its device and stream current, so that what the call allocates belongs to them."""
+    if stream is None:
+        return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    if stream.device.index != dev:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on cuda:{dev}")
+    return torch.cuda.stream(stream)
 
 
-def _opt(t):
-    return _p(t) if t is not None else None
+def _here(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 class PagedPlan:
@@ -207,27 +215,31 @@ class PagedPlan:
 
     def __init__(self, n_req: int, max_rows: int, device="cuda"):
         sizes = [n_req + 1, max_rows, max_rows, max_rows, n_req, 4]
-        parts = torch.empty(sum(sizes), dtype=torch.int32, device=device).split(sizes)
+        parts = torch.empty(sum(sizes), dtype=_I32, device=device).split(sizes)
         self.row_start, self.row_req, self.row_pos, self.slot_map, self.total_lens, self.status = parts
 
 
 def paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages: int, page_size: int, max_rows: int, pos0=0,
                plan: PagedPlan | None = None, stream=None) -> PagedPlan:
     """Block tables (in place) and the row tables of a step from the requests' lengths."""
-    i32, n = torch.int32, cached_lens.numel()
+    dev, n = _device(cached_lens), cached_lens.numel()
     if block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("block_table is [n_req, max_blocks], free_pages [n_free]")
-    _on(cached_lens, cached_lens=(cached_lens, i32, (n,)), new_lens=(new_lens, i32, (n,)), free_pages=(free_pages, i32, None),
-        block_table=(block_table, i32, (n, block_table.shape[1])))
-    with _Launch(cached_lens.device, stream) as st:
-        if plan is None:
-            plan = PagedPlan(n, max_rows, cached_lens.device)
-        _on(cached_lens, row_start=(plan.row_start, i32, (n + 1,)), row_req=(plan.row_req, i32, (max_rows,)),
-            row_pos=(plan.row_pos, i32, (max_rows,)), slot_map=(plan.slot_map, i32, (max_rows,)),
-            total_lens=(plan.total_lens, i32, (n,)), status=(plan.status, i32, (4,)))
-        check(lib().hyb_paged_plan(_p(cached_lens), _p(new_lens), n, page_size, n_pages, _p(free_pages), free_pages.numel(),
-                                   _p(block_table), block_table.shape[1], pos0, max_rows, _p(plan.row_start), _p(plan.row_req),
-                                   _p(plan.row_pos), _p(plan.slot_map), _p(plan.total_lens), _p(plan.status), st))
+    width, n_free = block_table.shape[1], free_pages.shape[0]
+    c, a = _ck("cached_lens", cached_lens, _I32, (n,), dev), _ck("new_lens", new_lens, _I32, (n,), dev)
+    f, b = _ck("free_pages", free_pages, _I32, (n_free,), dev), _ck("block_table", block_table, _I32, (n, width), dev)
+    ctx = _switch(dev, stream)
+    if ctx is not None:
+        with ctx:
+            return paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages, page_size, max_rows, pos0, plan)
+    if plan is None:
+        plan = PagedPlan(n, max_rows, cached_lens.device)
+    rows = (max_rows,)
+    check(lib().hyb_paged_plan(c, a, n, page_size, n_pages, f, n_free, b, width, pos0, max_rows,
+                               _ck("row_start", plan.row_start, _I32, (n + 1,), dev), _ck("row_req", plan.row_req, _I32, rows, dev),
+                               _ck("row_pos", plan.row_pos, _I32, rows, dev), _ck("slot_map", plan.slot_map, _I32, rows, dev),
+                               _ck("total_lens", plan.total_lens, _I32, (n,), dev), _ck("status", plan.status, _I32, (4,), dev),
+                               _here(dev)))
     return plan
 
 
@@ -235,29 +247,35 @@ def qkv_post_paged(qkv, n_heads, n_kv, hd, v_from_k, q_norm, k_norm, inv_freq, r
                    q_out=None, stream=None):
     """QK-norm, RoPE at row_pos and the cache write to slot_map of the pools [n_pages, page_size,
     n_kv, hd]; returns q [T, n_heads, hd]. qkv [T, ld] may have padded rows (its stride is used)."""
-    bf, i32 = torch.bfloat16, torch.int32
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.dtype != bf or (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
+    dev = _device(qkv)
+    if qkv.dim() != 2 or qkv.dtype is not _BF16 or qkv.stride(1) != 1:
         raise ValueError("qkv is bf16 [T, columns] with unit column stride")
-    T = qkv.shape[0]
-    if qkv.shape[1] < (n_heads + (1 if v_from_k else 2) * n_kv) * hd:
-        raise ValueError("qkv has fewer columns than q, k and v need")
-    if k_pool.dim() != 4 or k_pool.shape[2:] != (n_kv, hd):
+    T, cols = qkv.shape
+    ld = qkv.stride(0) if T > 1 else -(-cols // 8) * 8
+    if ld < cols or cols < (n_heads + (1 if v_from_k else 2) * n_kv) * hd:
+        raise ValueError("qkv has overlapping rows or fewer columns than q, k and v need")
+    shape = k_pool.shape
+    if len(shape) != 4 or shape[2] != n_kv or shape[3] != hd:
         raise ValueError("k_pool is [n_pages, page_size, n_kv, hd]")
-    _on(qkv, q_norm=(q_norm, bf, (hd,)), k_norm=(k_norm, bf, (hd,)), inv_freq=(inv_freq, torch.float32, (hd // 2,)),
-        row_pos=(row_pos, i32, (T,)), slot_map=(slot_map, i32, (T,)), k_pool=(k_pool, bf, None),
-        v_pool=(v_pool, bf, k_pool.shape), q_out=(q_out, bf, (T, n_heads, hd)))
-    with _Launch(qkv.device, stream) as st:
-        if q_out is None:
-            q_out = torch.empty((T, n_heads, hd), dtype=bf, device=qkv.device)
-        ld = qkv.stride(0) if T > 1 else -(-qkv.shape[1] // 8) * 8
-        check(lib().hyb_qkv_post_paged(_p(qkv), T, ld, n_heads, n_kv, hd, int(v_from_k), _p(q_norm), _p(k_norm), _p(inv_freq),
-                                       _p(row_pos), _p(slot_map), k_pool.shape[0] * k_pool.shape[1], eps, _p(q_out),
-                                       _p(k_pool), _p(v_pool), st))
+    ctx = _switch(dev, stream)
+    if ctx is not None:
+        with ctx:
+            return qkv_post_paged(qkv, n_heads, n_kv, hd, v_from_k, q_norm, k_norm, inv_freq, row_pos, slot_map, k_pool, v_pool,
+                                  eps, q_out)
+    if q_out is None:
+        q_out = torch.empty((T, n_heads, hd), dtype=_BF16, device=qkv.device)
+    check(lib().hyb_qkv_post_paged(qkv.data_ptr(), T, ld, n_heads, n_kv, hd, 1 if v_from_k else 0,
+                                   _ck("q_norm", q_norm, _BF16, (hd,), dev), _ck("k_norm", k_norm, _BF16, (hd,), dev),
+                                   _ck("inv_freq", inv_freq, _F32, (hd // 2,), dev), _ck("row_pos", row_pos, _I32, (T,), dev),
+                                   _ck("slot_map", slot_map, _I32, (T,), dev), shape[0] * shape[1], eps,
+                                   _ck("q_out", q_out, _BF16, (T, n_heads, hd), dev), _ck("k_pool", k_pool, _BF16, shape, dev),
+                                   _ck("v_pool", v_pool, _BF16, shape, dev), _here(dev)))
     return q_out
 
 
 class SharedPrefixScratch:
-    """Device workspace for sdpa_shared_prefix calls of at most these sizes (contents do not matter)."""
+    """Device workspace for sdpa_shared_prefix calls of these sizes (contents do not matter). A
+    larger one serves any call that needs no more bytes."""
 
     def __init__(self, T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd, device="cuda"):
         n = lib().hyb_sdpa_shared_prefix_scratch_bytes(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd)
@@ -271,48 +289,61 @@ def sdpa_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len: int, block_t
                        max_own: int, window=0, scale=1.0, softcap=0.0, scratch: SharedPrefixScratch | None = None, out=None,
                        stream=None):
     """Attention of rows q [T, H, hd] over the shared prefix and their requests' own pages."""
-    bf, i32 = torch.bfloat16, torch.int32
-    if q.dim() != 3 or k_pool.dim() != 4 or block_table.dim() != 2:
+    dev = _device(q)
+    shape = q.shape
+    if len(shape) != 3 or k_pool.dim() != 4 or block_table.dim() != 2:
         raise ValueError("q is [T, H, hd], the pools [n_pages, page_size, n_kv, hd], block_table [n_req, max_blocks]")
-    T, H, hd = q.shape
-    n_pages, page, nkv, _ = k_pool.shape
-    n = own_lens.numel()
-    _on(q, q=(q, bf, None), k_pool=(k_pool, bf, (n_pages, page, nkv, hd)), v_pool=(v_pool, bf, k_pool.shape),
-        prefix_table=(prefix_table, i32, None), block_table=(block_table, i32, (n, block_table.shape[1])),
-        own_lens=(own_lens, i32, (n,)), row_start=(row_start, i32, (n + 1,)), row_pos=(row_pos, i32, (T,)), out=(out, bf, q.shape))
+    T, H, hd = shape
+    pool = k_pool.shape
+    n_pages, page, nkv, _ = pool
+    n, width = own_lens.numel(), block_table.shape[1]
     if prefix_len < 0 or (prefix_len > 0 and (prefix_table is None or prefix_table.numel() * page < prefix_len)):
         raise ValueError("prefix_table does not hold prefix_len keys")
-    with _Launch(q.device, stream) as st:
-        if out is None:
-            out = torch.empty_like(q)
-        if scratch is None:
-            scratch = SharedPrefixScratch(T, n, max_q, max_own, prefix_len, H, nkv, hd, q.device)
-        _on(q, scratch=(scratch.buf, torch.uint8, None))
-        check(lib().hyb_sdpa_shared_prefix(_p(q), _p(k_pool), _p(v_pool), n_pages, page, _opt(prefix_table), prefix_len,
-                                           _p(block_table), block_table.shape[1], _p(own_lens), _p(row_start), _p(row_pos), T, n,
-                                           max_q, max_own, H, nkv, hd, window, scale, softcap, _p(out), _p(scratch.buf),
-                                           scratch.nbytes, st))
+    if pool[3] != hd:
+        raise ValueError(f"q has head_dim {hd}, the pools {pool[3]}")
+    ctx = _switch(dev, stream)
+    if ctx is not None:
+        with ctx:
+            return sdpa_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len, block_table, own_lens, row_start, row_pos,
+                                      max_q, max_own, window, scale, softcap, scratch, out)
+    L = lib()
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if scratch is None:
+        scratch = SharedPrefixScratch(T, n, max_q, max_own, prefix_len, H, nkv, hd, q.device)
+    if scratch.buf.get_device() != dev:
+        raise ValueError(f"scratch is on {scratch.buf.device}, expected cuda:{dev}")
+    check(L.hyb_sdpa_shared_prefix(_ck("q", q, _BF16, shape, dev), _ck("k_pool", k_pool, _BF16, pool, dev),
+                                   _ck("v_pool", v_pool, _BF16, pool, dev), n_pages, page,
+                                   None if prefix_table is None else _ck("prefix_table", prefix_table, _I32, (prefix_table.numel(),), dev),
+                                   prefix_len, _ck("block_table", block_table, _I32, (n, width), dev), width,
+                                   _ck("own_lens", own_lens, _I32, (n,), dev), _ck("row_start", row_start, _I32, (n + 1,), dev),
+                                   _ck("row_pos", row_pos, _I32, (T,), dev), T, n, max_q, max_own, H, nkv, hd, window, scale,
+                                   softcap, _ck("out", out, _BF16, shape, dev), scratch.buf.data_ptr(), scratch.nbytes, _here(dev)))
     return out
 
 
 def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None, stream=None):
     """(token, kept, prob) of every row of logits [rows, vocab] (bf16 or float32, rows may be
     padded), from uniforms u [rows] and per-row settings (None: off, temperature 1)."""
-    f32, i32 = torch.float32, torch.int32
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, f32) or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    dev, dtype = _device(logits), logits.dtype
+    if logits.dim() != 2 or (dtype is not _BF16 and dtype is not _F32) or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits is bf16 or float32 [rows, vocab] with unit column stride")
     n, V = logits.shape
-    if n > 1 and logits.stride(0) < V:
+    ld = logits.stride(0) if n > 1 else V
+    if ld < V:
         raise ValueError("the rows of logits overlap")
-    _on(logits, u=(u, f32, (n,)), temperature=(temperature, f32, (n,)), top_k=(top_k, i32, (n,)), top_p=(top_p, f32, (n,)),
-        min_p=(min_p, f32, (n,)))
-    with _Launch(logits.device, stream) as st:
-        if out is None:
-            out = (torch.empty(n, dtype=i32, device=logits.device), torch.empty(n, dtype=i32, device=logits.device),
-                   torch.empty(n, dtype=f32, device=logits.device))
-        token, kept, prob = out
-        _on(logits, token=(token, i32, (n,)), kept=(kept, i32, (n,)), prob=(prob, f32, (n,)))
-        check(lib().hyb_sample_batch(_p(logits), int(logits.dtype == f32), n, V, logits.stride(0) if n > 1 else V, _p(u),
-                                     _opt(temperature), _opt(top_k), _opt(top_p), _opt(min_p), _p(token), _p(kept), _p(prob),
-                                     st))
-    return token, kept, prob
+    rows = (n,)
+    args = (_ck("u", u, _F32, rows, dev), _ck_opt("temperature", temperature, _F32, rows, dev), _ck_opt("top_k", top_k, _I32, rows, dev),
+            _ck_opt("top_p", top_p, _F32, rows, dev), _ck_opt("min_p", min_p, _F32, rows, dev))
+    ctx = _switch(dev, stream)
+    if ctx is not None:
+        with ctx:
+            return sample_batch(logits, u, temperature, top_k, top_p, min_p, out)
+    if out is None:
+        whole = torch.empty((3, n), dtype=_I32, device=logits.device)
+        out = (whole[0], whole[1], whole[2].view(_F32))
+    token, kept, prob = out
+    check(lib().hyb_sample_batch(logits.data_ptr(), 1 if dtype is _F32 else 0, n, V, ld, *args, _ck("token", token, _I32, rows, dev),
+                                 _ck("kept", kept, _I32, rows, dev), _ck("prob", prob, _F32, rows, dev), _here(dev)))
+    return out

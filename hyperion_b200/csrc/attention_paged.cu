@@ -48,8 +48,7 @@ __device__ __forceinline__ void cp_wait() {
 
 constexpr int kTileRows = 16;
 constexpr int kWarps = 4;
-constexpr int kSlice = 16;             // keys of one warp step
-constexpr int kTargetCtas = 2 * 148;   // two waves of one CTA on every SM of a B200
+constexpr int kSlice = 16;  // keys of one warp step
 
 SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv) {
     SharedPlan s;
@@ -59,124 +58,150 @@ SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len,
     auto tiles = [](long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); };
     // Tiles of one request's rows when they fill 128-row tiles about as well as the whole
     // batch's rows do: then prefix and own keys are one pass.
-    const bool per_request = req_rows > kTileRows && 4ll * n_req * tiles(req_rows, kTcRows) <= 5ll * tiles(all_rows, kTcRows);
-    if (per_request) {
+    if (req_rows > kTileRows && 4ll * n_req * tiles(req_rows, kTcRows) <= 5ll * tiles(all_rows, kTcRows)) {
         s.tc_per_request = 1;
         s.tc_tiles = tiles(req_rows, kTcRows);
-    } else if (prefix_len > 0 && all_rows > kTileRows) {
+    } else if (prefix_len > 128 && all_rows > kTileRows) {
         s.tc_tiles = tiles(all_rows, kTcRows);
     }
     if (s.tc_tiles > 0) {
-        const long long units = static_cast<long long>(s.tc_tiles) * n_kv * (per_request ? n_req : 1);
-        const long long blocks = (prefix_len + (per_request ? max_own : 0) + 63) / 64;
+        const long long units = static_cast<long long>(s.tc_tiles) * n_kv * (s.tc_per_request ? n_req : 1);
+        const long long blocks = (static_cast<long long>(prefix_len) + (s.tc_per_request ? max_own : 0) + 63) / 64;
         s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((blocks + 1) / 2, 148 / units)));
-        if (per_request) return s;
-    } else if (prefix_len > 0) {
-        s.tiles_p = tiles(all_rows, kTileRows);
-        const long long units = static_cast<long long>(s.tiles_p) * n_kv;
-        s.split_p = static_cast<int>(std::max<long long>(1, std::min<long long>((prefix_len + 63) / 64, kTargetCtas / units)));
+        if (s.tc_per_request) return s;
     }
-    if (max_own > 0) {
-        s.tiles_o = tiles(req_rows, kTileRows);
-        const long long units = static_cast<long long>(s.tiles_o) * n_kv * n_req;
-        const long long want = std::max<long long>(1, std::min<long long>((max_own + 63) / 64, 2 * kTargetCtas / units));
-        s.chunk_o = static_cast<int>(((max_own + want - 1) / want + 63) / 64 * 64);
-        s.split_o = (max_own + s.chunk_o - 1) / s.chunk_o;
+    // A single request shares with nobody, and a short prefix costs less to read again than
+    // to treat apart.
+    s.o_prefix = s.tc_tiles == 0 && prefix_len > 0 && (n_req == 1 || prefix_len <= 128);
+    const bool prefix_items = s.tc_tiles == 0 && prefix_len > 0 && !s.o_prefix;
+    const long long keys_o = static_cast<long long>(max_own) + (s.o_prefix ? prefix_len : 0);
+    s.tiles_o = keys_o > 0 ? tiles(req_rows, kTileRows) : 0;
+    s.tiles_p = prefix_items ? tiles(all_rows, kTileRows) : 0;
+    // Parts of about the same length: as many as two CTAs on every SM take at once, of 64 to
+    // 1024 keys (a shorter part is all latency, a longer one leaves SMs idle at the end).
+    // Half of max_own stands for the requests' mean.
+    const long long units_o = static_cast<long long>(s.tiles_o) * n_kv * n_req, units_p = static_cast<long long>(s.tiles_p) * n_kv;
+    const long long work = units_o * (s.o_prefix ? prefix_len + max_own / 2 : max_own / 2) + units_p * prefix_len;
+    const long long part = std::min<long long>(1024, std::max<long long>(64, (work / 296 + 63) / 64 * 64));
+    if (s.tiles_p > 0) s.split_p = static_cast<int>((prefix_len + part - 1) / part);
+    if (s.tiles_o > 0) {
+        s.chunk_o = static_cast<int>(part / kSlice);
+        s.split_o = static_cast<int>(((prefix_len * (s.o_prefix ? 1ll : 0ll) + kSlice - 1) / kSlice + (max_own + kSlice - 1) / kSlice + s.chunk_o - 1) / s.chunk_o);
     }
     return s;
 }
 
+// The keys of one segment (prefix or own) for a tile of rows: those in [lo, hi) are seen by some
+// row, its slices start at key `first`.
+struct Keys {
+    const int* table;
+    int base, lo, hi, first, slices;
+};
+__device__ __forceinline__ Keys keys_of(const int* table, int base, int len, int pmin, int pmax, int window) {
+    Keys k;
+    k.table = table;
+    k.base = base;
+    k.hi = static_cast<int>(min(static_cast<long long>(len), max(0ll, static_cast<long long>(pmax) + 1 - base)));
+    k.lo = 0;
+    if (window > 0) k.lo = static_cast<int>(min(static_cast<long long>(k.hi), max(0ll, static_cast<long long>(pmin) - window + 1 - base)));
+    k.first = k.lo & ~(kSlice - 1);
+    // without a window the slices depend on the length alone, so that their pages can be looked
+    // up before the rows' positions are known
+    k.slices = window > 0 ? (k.hi > k.lo ? (k.hi - k.first + kSlice - 1) / kSlice : 0) : (len + kSlice - 1) / kSlice;
+    return k;
+}
+
 template <int HD>
 struct SmallPlan {
-    static constexpr int kStages = 3;
-    static constexpr int kHalf = kSlice * HD * 2;          // K or V of one slice
-    static constexpr int kStage = 2 * kHalf;
-    static constexpr int kRing = kWarps * kStages * kStage;
+    // K or V of one slice is one stage; 24 KB a warp (12 KB for head_dim 64), so that two CTAs
+    // (four) share an SM and one streams while the other starts or ends
+    static constexpr int kHalf = kSlice * HD * 2;
+    static constexpr int kStages = HD == 256 ? 3 : 6;
+    static constexpr int kRing = kWarps * kStages * kHalf;
     static constexpr int kMerge = kWarps * kTileRows * HD * 4;
     static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
 };
 
 // One CTA: up to 16 rows (row m of a tile = token m / G, head m % G of the KV head's group)
-// against one part of the prefix or of one request's keys. Each warp takes every fourth
-// 16-key slice of the part on its own: cp.async into its own 3-stage ring (zero fill of keys
-// that no row of the tile sees, so whatever the pool holds there cannot reach a product),
-// QK^T and PV on mma.sync m16n8k16, online softmax; the four warps' results are joined at
-// the end. Rows share every byte of K and V that is loaded, so up to 16 rows cost the same
-// traffic as one: HBM bound.
+// against one part of the prefix, or of one request's keys. Each warp takes every fourth
+// 16-key slice of the part on its own: cp.async into its own ring (zero fill of keys that no
+// row of the tile sees, so whatever the pool holds there cannot reach a product), QK^T and PV
+// on mma.sync m16n8k16, online softmax; the four warps' results are joined at the end. Rows
+// share every byte of K and V that is loaded, so up to 16 rows cost the same traffic as one:
+// HBM bound. The chain in front of the first copy is three loads deep: lengths, row starts
+// and pages; positions; keys.
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const SharedAttnParams p, const SharedPlan pl,
-                                                                        SharedParts parts) {
+__global__ void __launch_bounds__(kWarps * 32, 2) shared_attn_small_kernel(const SharedAttnParams p, const SharedPlan pl,
+                                                                           SharedParts parts, int after_tc) {
     using SP = SmallPlan<HD>;
-    constexpr int KS = HD / 16, CH = HD / 8;
+    constexpr int KS = HD / 16, CH = HD / 8, ST = SP::kStages;
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ float s_m[kWarps][kTileRows], s_l[kWarps][kTileRows];
-    __shared__ int s_pos[kTileRows];
+    __shared__ int s_row[kTileRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.n_heads / p.n_kv;
+    pdl_launch_dependents();
 
     // ---- which part
-    long long id = blockIdx.x;
-    const long long n_prefix = static_cast<long long>(pl.tiles_p) * p.n_kv * pl.split_p;
+    int id = blockIdx.x;
+    const int n_prefix = pl.tiles_p * p.n_kv * pl.split_p;
     const bool prefix = id < n_prefix;
     int split, hk, tile, req = 0;
     if (prefix) {
-        split = static_cast<int>(id % pl.split_p);
+        split = id % pl.split_p;
         id /= pl.split_p;
-        hk = static_cast<int>(id % p.n_kv);
-        tile = static_cast<int>(id / p.n_kv);
+        hk = id % p.n_kv;
+        tile = id / p.n_kv;
     } else {
         id -= n_prefix;
-        hk = static_cast<int>(id % p.n_kv);
+        hk = id % p.n_kv;
         id /= p.n_kv;
-        split = static_cast<int>(id % pl.split_o);
+        split = id % pl.split_o;
         id /= pl.split_o;
-        tile = static_cast<int>(id % pl.tiles_o);
-        req = static_cast<int>(id / pl.tiles_o);
+        tile = id % pl.tiles_o;
+        req = id / pl.tiles_o;
     }
-    // ---- its rows: m in [m0, m0 + rows) of the (token, head) pairs from token t0 on
-    int t0 = 0, n_tok = p.T;
+    // ---- lengths, row starts
+    int t0 = 0, n_tok = p.T, own = 0;
+    const long long most = min(static_cast<long long>(p.max_own), static_cast<long long>(p.max_blocks) * p.page_size);
+    bool broken = false;
     if (!prefix) {
-        t0 = min(max(p.row_start[req], 0), p.T);
-        n_tok = min(min(p.row_start[req + 1], p.T) - t0, p.max_q);
+        const int a = p.row_start[req], b = p.row_start[req + 1], len = p.own_lens[req];
+        t0 = min(max(a, 0), p.T);
+        n_tok = min(min(b, p.T) - t0, p.max_q);
+        own = static_cast<int>(min(static_cast<long long>(max(0, len)), most));
+        broken = len > most;
     }
-    const long long m0 = static_cast<long long>(tile) * kTileRows;
+    const int len_p = prefix || pl.o_prefix ? p.prefix_len : 0;
+    const int per = prefix ? 0 : pl.chunk_o;
+    const int* own_table = p.table + static_cast<size_t>(req) * p.max_blocks;
+    // ---- the pages of this warp's first 32 slices, one a lane, while no window moves the slices
+    int pages = 0;
+    const int slices_p = (len_p + kSlice - 1) / kSlice;
+    // a prefix item splits the prefix evenly, in steps of 64 keys
+    const int per_p = prefix ? (((p.prefix_len + pl.split_p - 1) / pl.split_p + 63) & ~63) / kSlice : 0;
+    if (p.window == 0) {
+        const int s = split * (prefix ? per_p : per) + warp + lane * kWarps;
+        if (s < slices_p) pages = p.prefix_table[s * kSlice / p.page_size];
+        else if (!prefix && s - slices_p < (own + kSlice - 1) / kSlice) pages = own_table[(s - slices_p) * kSlice / p.page_size];
+    }
+    if (parts.direct && tile == pl.tiles_o - 1 && split == 0) shared_fill_unserved(p, req, hk, t0, kWarps * 32);
+    // ---- rows m0 .. m0 + rows of the (token, head) pairs from token t0 on
+    const int m0 = tile * kTileRows;
     const int rows = static_cast<int>(max(0ll, min(static_cast<long long>(kTileRows), static_cast<long long>(n_tok) * G - m0)));
-    if (rows <= 0) return;
-    if (threadIdx.x < kTileRows)
-        s_pos[threadIdx.x] = threadIdx.x < rows ? p.row_pos[t0 + (m0 + threadIdx.x) / G] : -1;
-    __syncthreads();
-    int pmin = INT_MAX, pmax = -1;
-#pragma unroll
-    for (int m = 0; m < kTileRows; ++m)
-        if (s_pos[m] >= 0) {
-            pmin = min(pmin, s_pos[m]);
-            pmax = max(pmax, s_pos[m]);
-        }
-    // ---- its keys: [lo, hi) are seen by some row, [k0, k1) are this part's
-    const int base = prefix ? 0 : p.prefix_len;
-    const long long table_keys = static_cast<long long>(p.max_blocks) * p.page_size;
-    const int len = prefix ? p.prefix_len
-                           : static_cast<int>(min(static_cast<long long>(max(0, min(p.own_lens[req], p.max_own))), table_keys));
-    const int hi = min(len, max(0, pmax + 1 - base));
-    const int lo = p.window > 0 && pmax >= 0
-                       ? static_cast<int>(min(static_cast<long long>(hi), max(0ll, static_cast<long long>(pmin) - p.window + 1 - base)))
-                       : 0;
-    const int first = lo & ~(kSlice - 1);  // parts start on slice borders
-    const int per = prefix ? ((hi - first + pl.split_p - 1) / pl.split_p + 63) & ~63 : pl.chunk_o;
-    const long long from = first + static_cast<long long>(split) * per;
-    const int k0 = static_cast<int>(min(from, static_cast<long long>(hi))), k1 = static_cast<int>(min(from + per, static_cast<long long>(hi)));
-    const int* table = prefix ? p.prefix_table : p.table + static_cast<size_t>(req) * p.max_blocks;
-    const int n_slices = k1 > k0 ? (k1 - k0 + kSlice - 1) / kSlice : 0;
-    const int mine = n_slices > warp ? (n_slices - warp + kWarps - 1) / kWarps : 0;
-
-    // ---- queries into fragments
-    uint32_t qf[KS][4];
+    if (rows <= 0) {
+        if (after_tc) pdl_wait();
+        return;
+    }
+    // lane m (and m + 16): row m's position and place
+    const int mm = m0 + min(lane & 15, rows - 1), tok = mm / G;
+    const int my_pos = (lane & 15) < rows ? p.row_pos[t0 + tok] : -1;
+    const int my_row = (t0 + tok) * p.n_heads + hk * G + (mm - tok * G);
     const int g = lane >> 2, c2 = 2 * (lane & 3);
+    uint32_t qf[KS][4];
     {
-        const int mA = g, mB = g + 8;
-        const long long pa = m0 + min(mA, rows - 1), pb = m0 + min(mB, rows - 1);
-        const bf16* qa = p.q + ((t0 + pa / G) * p.n_heads + hk * G + pa % G) * HD;
-        const bf16* qb = p.q + ((t0 + pb / G) * p.n_heads + hk * G + pb % G) * HD;
+        const bf16* qa = p.q + static_cast<size_t>(__shfl_sync(0xffffffffu, my_row, g)) * HD;
+        const bf16* qb = p.q + static_cast<size_t>(__shfl_sync(0xffffffffu, my_row, g + 8)) * HD;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             qf[k][0] = *reinterpret_cast<const uint32_t*>(qa + 16 * k + c2);
@@ -185,7 +210,19 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
             qf[k][3] = *reinterpret_cast<const uint32_t*>(qb + 16 * k + 8 + c2);
         }
     }
-    const int posA = s_pos[g], posB = s_pos[g + 8];
+    if (warp == 0 && lane < kTileRows) s_row[lane] = my_row | (my_pos < 0 ? 0x80000000 : 0);
+    const int pmin = __reduce_min_sync(0xffffffffu, my_pos < 0 ? INT_MAX : my_pos);
+    const int pmax = __reduce_max_sync(0xffffffffu, my_pos);
+    const int posA = __shfl_sync(0xffffffffu, my_pos, g), posB = __shfl_sync(0xffffffffu, my_pos, g + 8);
+    // ---- its keys: slices [s0, s1) of the prefix's, then the request's own
+    const Keys ka = keys_of(p.prefix_table, 0, len_p, pmin, pmax, p.window);
+    const Keys kb = keys_of(own_table, p.prefix_len, own, pmin, pmax, p.window);
+    const int total = ka.slices + kb.slices;
+    const int step = !prefix ? per : (p.window == 0 ? per_p : (ka.slices + pl.split_p - 1) / pl.split_p);
+    const int s0 = static_cast<int>(min(static_cast<long long>(total), static_cast<long long>(split) * step));
+    const int s1 = min(total, s0 + step);
+    const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kWarps - 1) / kWarps : 0;
+
     float o[HD / 8][4];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i)
@@ -194,72 +231,87 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
     float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
     bool bad = false;
 
-    const uint32_t ring = smem_u32(sm) + warp * SP::kStages * SP::kStage;
-    int pages = 0;  // lane i: the page of this warp's slice i of the current 32
-    auto load_pages = [&](int from) {
-        const int i = from + lane;
-        const int key = k0 + (warp + i * kWarps) * kSlice;
-        pages = i < mine ? table[key / p.page_size] : 0;
-        if (pages < 0 || pages >= p.n_pages) {
+    const uint32_t ring = smem_u32(sm) + warp * ST * SP::kHalf;
+    auto load_pages = [&](int from) {  // of this warp's slices from .. from + 31
+        const int i = from + lane, s = s0 + warp + i * kWarps;
+        if (from > 0 || p.window > 0) {
+            pages = 0;
+            if (i < mine) {
+                const bool a = s < ka.slices;
+                pages = (a ? ka.table : kb.table)[(a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice) / p.page_size];
+            }
+        }
+        if (i < mine && (pages < 0 || pages >= p.n_pages)) {
             bad = true;
             pages = -1;
         }
     };
-    auto fetch = [&](int i) {  // this warp's slice i into stage i % kStages
+    int f_slot = 0;
+    auto fetch = [&](int j) {  // K (even) or V (odd) of this warp's slice j / 2
+        const int i = j >> 1;
         if (i < mine) {
-            if ((i & 31) == 0) load_pages(i);
+            if ((j & 63) == 0) load_pages(i);
             const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-            const int key0 = k0 + (warp + i * kWarps) * kSlice;
+            const int s = s0 + warp + i * kWarps;
+            const bool a = s < ka.slices;
+            const int key0 = a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
+            const int lo = a ? ka.lo : kb.lo, hi = a ? ka.hi : kb.hi;
             const size_t cell = (static_cast<size_t>(max(page, 0)) * p.page_size + key0 % p.page_size) * p.n_kv + hk;
-            const bf16* kg = p.k_pool + cell * HD;
-            const bf16* vg = p.v_pool + cell * HD;
-            const uint32_t dst = ring + (i % SP::kStages) * SP::kStage;
-            const size_t step = static_cast<size_t>(p.n_kv) * HD;
+            const bf16* src = ((j & 1) ? p.v_pool : p.k_pool) + cell * HD;
+            const uint32_t dst = ring + f_slot * SP::kHalf;
+            const size_t row = static_cast<size_t>(p.n_kv) * HD;
+            constexpr int KPI = 32 / CH > 0 ? 32 / CH : 1;  // keys of one instruction
+            const int k_lane = lane / CH, ch = lane % CH;
+            const int from = lo - key0, to = page >= 0 ? hi - key0 : 0;
+            src += k_lane * row + ch * 8;
 #pragma unroll
-            for (int j = 0; j < kSlice * CH / 32; ++j) {
-                const int idx = lane + 32 * j, key = idx / CH, ch = idx % CH;
-                const bool take = page >= 0 && key0 + key >= lo && key0 + key < hi;
-                const uint32_t at = dst + key * (HD * 2) + ((ch ^ (key & 7)) << 4);
-                cp16(at, kg + (take ? key * step + ch * 8 : 0), take);
-                cp16(at + SP::kHalf, vg + (take ? key * step + ch * 8 : 0), take);
+            for (int q = 0; q < kSlice / KPI; ++q) {
+                const int key = q * KPI + k_lane;
+                cp16(dst + key * (HD * 2) + ((ch ^ (key & 7)) << 4), src + q * KPI * row, key >= from && key < to);
             }
         }
         cp_commit();
+        f_slot = f_slot + 1 == ST ? 0 : f_slot + 1;
     };
 #pragma unroll
-    for (int i = 0; i < SP::kStages - 1; ++i) fetch(i);
+    for (int j = 0; j < ST - 1; ++j) fetch(j);
     const float scale2 = p.scale * kSharedLog2e;
+    int slot = 0;
     for (int i = 0; i < mine; ++i) {
-        fetch(i + SP::kStages - 1);
-        cp_wait<SP::kStages - 1>();
+        fetch(2 * i + ST - 1);
+        cp_wait<ST - 1>();
         __syncwarp();
-        const uint32_t kb = ring + (i % SP::kStages) * SP::kStage, vb = kb + SP::kHalf;
-        const int key0 = k0 + (warp + i * kWarps) * kSlice;
+        const uint32_t kt = ring + slot * SP::kHalf;
+        slot = slot + 1 == ST ? 0 : slot + 1;
+        const int s = s0 + warp + i * kWarps;
+        const bool in_a = s < ka.slices;
+        const int key0 = in_a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
+        const int lo = in_a ? ka.lo : kb.lo, hi = in_a ? ka.hi : kb.hi, base = in_a ? 0 : p.prefix_len;
         // scores of 16 rows x 16 keys: this lane's rows g, g + 8 and keys c2, c2 + 1 (+ 8)
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        float s0v[4] = {0.f, 0.f, 0.f, 0.f}, s1v[4] = {0.f, 0.f, 0.f, 0.f};
         {
             const int key = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t b0, b1, b2, b3;
-                ldsm_x4(kb + key * (HD * 2) + (((2 * k + half) ^ (key & 7)) << 4), b0, b1, b2, b3);
-                mma_bf16_16816(s0, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b0, b1);
-                mma_bf16_16816(s1, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b2, b3);
+                ldsm_x4(kt + key * (HD * 2) + (((2 * k + half) ^ (key & 7)) << 4), b0, b1, b2, b3);
+                mma_bf16_16816(s0v, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b0, b1);
+                mma_bf16_16816(s1v, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b2, b3);
             }
         }
         auto shape = [&](float dot, int key, int pos) {
-            float s = p.softcap > 0.f ? p.softcap * kSharedLog2e * tanhf(dot * p.scale / p.softcap) : dot * scale2;
+            const float sc = p.softcap > 0.f ? p.softcap * kSharedLog2e * tanhf(dot * p.scale / p.softcap) : dot * scale2;
             const int kp = base + key;
             const bool see = key >= lo && key < hi && kp <= pos && (p.window == 0 || kp > pos - p.window);
-            return see ? s : -INFINITY;
+            return see ? sc : -INFINITY;
         };
         float v[8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            v[j] = shape(s0[j], key0 + c2 + j, posA);
-            v[2 + j] = shape(s1[j], key0 + 8 + c2 + j, posA);
-            v[4 + j] = shape(s0[2 + j], key0 + c2 + j, posB);
-            v[6 + j] = shape(s1[2 + j], key0 + 8 + c2 + j, posB);
+            v[j] = shape(s0v[j], key0 + c2 + j, posA);
+            v[2 + j] = shape(s1v[j], key0 + 8 + c2 + j, posA);
+            v[4 + j] = shape(s0v[2 + j], key0 + c2 + j, posB);
+            v[6 + j] = shape(s1v[2 + j], key0 + 8 + c2 + j, posB);
         }
         float xA = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), xB = fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]));
 #pragma unroll
@@ -293,17 +345,23 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
             if (j < 2) lA += sum;
             else lB += sum;
         }
+        __syncwarp();  // every lane has read the K stage that the next fetch refills
+        fetch(2 * i + ST);
+        cp_wait<ST - 1>();
+        __syncwarp();
+        const uint32_t vt = ring + slot * SP::kHalf;
+        slot = slot + 1 == ST ? 0 : slot + 1;
         {
             const int key = lane & 15, half = lane >> 4;
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) {
                 uint32_t b0, b1, b2, b3;
-                ldsm_x4_t(vb + key * (HD * 2) + (((2 * d + half) ^ (key & 7)) << 4), b0, b1, b2, b3);
+                ldsm_x4_t(vt + key * (HD * 2) + (((2 * d + half) ^ (key & 7)) << 4), b0, b1, b2, b3);
                 mma_bf16_16816(o[2 * d], pf[0], pf[2], pf[1], pf[3], b0, b1);
                 mma_bf16_16816(o[2 * d + 1], pf[0], pf[2], pf[1], pf[3], b2, b3);
             }
         }
-        __syncwarp();  // every lane has read the stage that the next fetch refills
+        __syncwarp();  // and the V stage
     }
     cp_wait<0>();
 #pragma unroll
@@ -312,7 +370,7 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
         lB += __shfl_xor_sync(0xffffffffu, lB, w);
     }
     // a page outside the pool: the rows of the tile come out as NaN, not as a silent subset
-    if (__any_sync(0xffffffffu, bad)) {
+    if (__any_sync(0xffffffffu, bad) || (broken && parts.direct)) {
         lA = lB = __int_as_float(0x7fffffff);
         mA = mB = 0.f;
     }
@@ -349,78 +407,123 @@ __global__ void __launch_bounds__(kWarps * 32) shared_attn_small_kernel(const Sh
             acc.z += f * x.z;
             acc.w += f * x.w;
         }
-        const long long pr = m0 + m;
-        const size_t row = static_cast<size_t>(t0 + pr / G) * p.n_heads + hk * G + pr % G;
-        if (L != 0.f) *reinterpret_cast<float4*>(parts.o + (row * parts.n + at) * HD + d) = acc;
-        if (d == 0) parts.ml[row * parts.n + at] = make_float2(M, L);
+        const size_t row = static_cast<size_t>(s_row[m] & 0x7fffffff);
+        if (!parts.direct) {
+            if (L != 0.f) *reinterpret_cast<float4*>(parts.o + (row * parts.n + at) * HD + d) = acc;
+            if (d == 0) parts.ml[row * parts.n + at] = make_float2(M, L);
+        } else if (s_row[m] >= 0) {  // the only part of its rows: the output itself
+            const float inv = L > 0.f ? 1.0f / L : L;
+            *reinterpret_cast<uint2*>(p.out + row * HD + d) =
+                make_uint2(pack_bf2(f2bf(acc.x * inv), f2bf(acc.y * inv)), pack_bf2(f2bf(acc.z * inv), f2bf(acc.w * inv)));
+        }
     }
+    // this grid may start under the 128-row kernel's last CTAs; it ends after them, so that the
+    // merge, which waits for this grid, waits for both
+    if (after_tc) pdl_wait();
 }
 
-// One warp per (row, head): joins the parts. Rows before row_start[0] or from
+// W warps per (row, head) join its parts, each every W-th. Rows before row_start[0] or from
 // row_start[n_req] on belong to no request and are left as they were; a row whose request
 // breaks the bounds the caller gave (more rows than max_q, more keys than max_own or its
 // table) has parts that were not computed and becomes NaN.
 template <int HD>
-__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParams p, SharedParts parts) {
-    const int lane = threadIdx.x & 31;
-    const long long unit = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (unit >= static_cast<long long>(p.T) * p.n_heads) return;
-    const int t = static_cast<int>(unit / p.n_heads);
-    if (t < p.row_start[0] || t >= p.row_start[p.n_req] || p.row_pos[t] < 0) return;
-    int lo = 0, hi = p.n_req;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.row_start[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const int own = p.own_lens[lo];
-    const bool broken = t - p.row_start[lo] >= p.max_q || own > p.max_own ||
-                        own > static_cast<long long>(p.max_blocks) * p.page_size;
-    const int splits = parts.n;
-    const float2* ml = parts.ml + unit * splits;
-    const float* src = parts.o + unit * splits * HD;
-    float M = -INFINITY;
-    for (int s = lane; s < splits; s += 32) M = fmaxf(M, ml[s].x);
-    M = warp_max(M);
-    const float z = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParams p, SharedParts parts, int W) {
     constexpr int PER = HD / 32;
-    float acc[PER];
+    __shared__ float s_o[8][HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % W;
+    const long long unit = (static_cast<long long>(blockIdx.x) * 8 + warp) / W;
+    const int t = static_cast<int>(min(unit / p.n_heads, static_cast<long long>(p.T)));
+    bool live = t < p.T, broken = false;
+    if (live) {
+        live = t >= p.row_start[0] && t < p.row_start[p.n_req] && p.row_pos[t] >= 0;
+        if (live) {
+            int lo = 0, hi = p.n_req;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (p.row_start[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            const int own = p.own_lens[lo];
+            broken = t - p.row_start[lo] >= p.max_q || own > p.max_own ||
+                     own > static_cast<long long>(p.max_blocks) * p.page_size;
+        }
+    }
+    pdl_wait();
+    float L = 0.f, acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float2 v = ml[s];
-        if (v.y == 0.f) continue;  // no key of the part is seen
-        const float f = shared_ex2(v.x - z);
-        L += f * v.y;
+    if (live) {
+        const float2* ml = parts.ml + static_cast<size_t>(unit) * parts.n;
+        const float* src = parts.o + static_cast<size_t>(unit) * parts.n * HD + lane * PER;
+        float M = -INFINITY;
+        for (int s = lane; s < parts.n; s += 32) M = fmaxf(M, ml[s].x);
+        M = warp_max(M);
+        const float z = M == -INFINITY ? 0.f : M;
+        for (int s0 = 0; s0 < parts.n; s0 += 32) {
+            float f = 0.f, fl = 0.f;
+            if (s0 + lane < parts.n) {
+                const float2 v = ml[s0 + lane];
+                f = v.y == 0.f ? 0.f : shared_ex2(v.x - z);  // l = 0: no key of the part is seen, no output written
+                fl = f * v.y;
+            }
+            L += warp_sum(fl);
+            const int n = min(32, parts.n - s0);
+#pragma unroll 4
+            for (int s = sub; s < n; s += W) {
+                const float fs = __shfl_sync(0xffffffffu, f, s);
+                if (fs == 0.f) continue;
+                const float* at = src + static_cast<size_t>(s0 + s) * HD;
+                if constexpr (PER == 2) {
+                    const float2 x = *reinterpret_cast<const float2*>(at);
+                    acc[0] += fs * x.x;
+                    acc[1] += fs * x.y;
+                } else {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] += f * src[static_cast<size_t>(s) * HD + lane * PER + i];
+                    for (int i = 0; i < PER; i += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(at + i);
+                        acc[i] += fs * x.x;
+                        acc[i + 1] += fs * x.y;
+                        acc[i + 2] += fs * x.z;
+                        acc[i + 3] += fs * x.w;
+                    }
+                }
+            }
+        }
     }
+    if (W > 1) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s_o[warp][lane * PER + i] = acc[i];
+        __syncthreads();
+        if (sub != 0) return;
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) acc[i] += s_o[warp + w][lane * PER + i];
+    }
+    if (!live) return;
     float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // no key seen: zeros; NaN stays
     if (broken) inv = __int_as_float(0x7fffffff);
-    uint32_t w[PER / 2];
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(unit) * HD + lane * PER);
 #pragma unroll
-    for (int i = 0; i < PER / 2; ++i) w[i] = pack_bf2(f2bf(acc[2 * i] * inv), f2bf(acc[2 * i + 1] * inv));
-    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + unit * HD + lane * PER);
-#pragma unroll
-    for (int i = 0; i < PER / 2; ++i) dst[i] = w[i];
+    for (int i = 0; i < PER / 2; ++i) dst[i] = pack_bf2(f2bf(acc[2 * i] * inv), f2bf(acc[2 * i + 1] * inv));
 }
 
 template <int HD>
-void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, SharedParts parts, cudaStream_t stream) {
+void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream) {
     using SP = SmallPlan<HD>;
     const long long n_prefix = static_cast<long long>(pl.tiles_p) * p.n_kv * pl.split_p;
-    const long long n_own = static_cast<long long>(pl.tiles_o) * p.n_kv * pl.split_o * p.n_req;
-    if (pl.tc_splits > 0) launch_shared_attn_tc(p, pl, parts, stream);
-    if (n_prefix + n_own > INT_MAX) throw ArgError("sdpa_shared_prefix: too many parts");
-    if (n_prefix + n_own > 0) {
-        allow_smem(reinterpret_cast<const void*>(shared_attn_small_kernel<HD>), SP::kSmem);
-        shared_attn_small_kernel<HD><<<static_cast<unsigned>(n_prefix + n_own), kWarps * 32, SP::kSmem, stream>>>(p, pl, parts);
-        HYB_LAUNCH_CHECK("shared_attn_small_kernel");
-    }
+    const long long n_req = static_cast<long long>(pl.tiles_o) * p.n_kv * pl.split_o * p.n_req;
     const long long warps = static_cast<long long>(p.T) * p.n_heads;
-    shared_merge_kernel<HD><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(p, parts);
-    HYB_LAUNCH_CHECK("shared_merge_kernel");
+    if (n_prefix + n_req > INT_MAX || warps > INT_MAX - 8) throw ArgError("sdpa_shared_prefix: too many parts");
+    if (pl.tc_splits > 0) launch_shared_attn_tc(p, pl, parts, stream);
+    if (n_prefix + n_req > 0) {
+        allow_smem(reinterpret_cast<const void*>(shared_attn_small_kernel<HD>), SP::kSmem);
+        shared_launch(shared_attn_small_kernel<HD>, static_cast<unsigned>(n_prefix + n_req), kWarps * 32, SP::kSmem, stream,
+                      pl.tc_splits > 0, p, pl, parts, pl.tc_splits > 0 ? 1 : 0);
+    }
+    if (parts.direct) return;  // the only part wrote the output
+    // one warp joins a few parts as fast as several: the loads of four are in flight at once
+    const int W = parts.n >= 16 ? 8 : (parts.n >= 8 ? 4 : (parts.n >= 4 ? 2 : 1));
+    shared_launch(shared_merge_kernel<HD>, static_cast<unsigned>((warps * W + 7) / 8), 256, 0, stream, parts.n > 0, p, parts, W);
 }
 
 }  // namespace
@@ -428,8 +531,8 @@ void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, SharedPart
 size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
                                  int hd) {
     const SharedPlan s = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv);
-    const size_t units = static_cast<size_t>(T) * n_heads * s.splits();
-    return units * hd * sizeof(float) + units * sizeof(float2) + 16;
+    const size_t units = s.direct() ? 0 : static_cast<size_t>(T) * n_heads * s.splits();
+    return units * hd * sizeof(float) + units * sizeof(float2) + 512;
 }
 
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
@@ -438,9 +541,10 @@ void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
     if (p.scratch_bytes < shared_attn_scratch_bytes(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd))
         throw ArgError("sdpa_shared_prefix: scratch too small");
     SharedParts parts;
-    parts.o = static_cast<float*>(p.scratch);
+    parts.o = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(p.scratch) + 255) & ~static_cast<uintptr_t>(255));
     parts.ml = reinterpret_cast<float2*>(parts.o + units * p.hd);
     parts.n = pl.splits();
+    parts.direct = pl.direct();
     switch (p.hd) {
         case 64: launch_shared_t<64>(p, pl, parts, stream); break;
         case 128: launch_shared_t<128>(p, pl, parts, stream); break;

@@ -4,6 +4,8 @@
 
 #include "kernels.h"
 
+#include <utility>
+
 namespace hyb {
 
 constexpr float kSharedLog2e = 1.4426950408889634f;
@@ -23,9 +25,12 @@ struct SharedPlan {
     int tc_tiles = 0;        // 128-row tiles over all rows, or of one request
     int tc_per_request = 0;  // tiles hold one request's rows and cover prefix and own keys
     int tiles_p = 0, split_p = 0;  // 16-row tiles over all rows; parts of the prefix
-    int tiles_o = 0, split_o = 0;  // 16-row tiles of one request; parts of its own keys
-    int chunk_o = 0;               // own keys of one part
+    int tiles_o = 0, split_o = 0;  // 16-row tiles of one request; parts of its keys
+    int chunk_o = 0;               // 16-key slices of one part
+    int o_prefix = 0;              // a request's 16-row tiles cover the prefix too
     __host__ __device__ int splits() const { return tc_splits + split_p + split_o; }
+    // one part, of tiles that hold the rows of one request: it writes the output itself
+    bool direct() const { return splits() == 1 && (tc_per_request != 0 || split_o == 1); }
 };
 
 // Scratch: fp32 partial outputs [T][n_heads][n][hd], then (m, l) pairs [T][n_heads][n]; m in
@@ -34,7 +39,35 @@ struct SharedParts {
     float* o;
     float2* ml;
     int n;
+    int direct;  // no scratch and no merge
 };
+
+// Rows of request `req` at or past max_q (no tile holds them): NaN, in the heads of one KV head.
+// For calls without a merge, by one CTA of the request.
+__device__ __forceinline__ void shared_fill_unserved(const SharedAttnParams& p, int req, int hk, int t0, int threads) {
+    const int t1 = min(p.row_start[req + 1], p.T), G = p.n_heads / p.n_kv;
+    for (int t = max(t0, t0 + min(p.max_q, p.T)); t < t1; ++t) {
+        if (p.row_pos[t] < 0) continue;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + (static_cast<size_t>(t) * p.n_heads + hk * G) * p.hd);
+        for (int i = threadIdx.x; i < G * p.hd / 2; i += threads) dst[i] = 0x7fff7fffu;
+    }
+}
+
+// Launch with an optional programmatic dependency on the kernel before it in the stream.
+template <typename... P, typename... A>
+void shared_launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, bool pdl, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    HYB_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...));
+}
 
 void launch_shared_attn_tc(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream);
 

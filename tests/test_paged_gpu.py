@@ -348,6 +348,17 @@ def test_attn_prefill_rows(built_lib, hd):
     b.check(b.call(), rows=[0, 1, 31, 32, 63, 64, 149, 150, 250, 282, 283])
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attn_many_blocks(built_lib, hd):
+    """Hundreds of key blocks in one pass, with and without parts, and several tiles per SM."""
+    b = Batch(16, 8, hd, 128, 3001, [64] * 40, [64] * 40, seed=hd)  # 320 tiles, one part each
+    b.check(b.call(), rows=[0, 63, 64, 1281, 2559])
+    b = Batch(4, 2, hd, 64, 20011, [80, 100], [64, 64], seed=hd + 1)  # few tiles, many parts
+    b.check(b.call(), rows=[0, 1, 63, 64, 127])
+    b = Batch(150, 150, hd, 256, 6000, [64], [64], seed=hd + 2)  # 150 heads: one long part each
+    b.check(b.call(), rows=[0, 63])
+
+
 def test_attn_scores_far_apart(built_lib):
     """Scores of some hundreds, growing along the keys (every tile moves the maximum) and falling."""
     for order in (1, -1):

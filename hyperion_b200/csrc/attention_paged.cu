@@ -50,7 +50,7 @@ constexpr int kTileRows = 16;
 constexpr int kWarps = 4;
 constexpr int kSlice = 16;  // keys of one warp step
 
-SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv) {
+SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv, int hd) {
     SharedPlan s;
     const int G = n_heads / n_kv;
     max_q = std::min(max_q, T);
@@ -77,9 +77,9 @@ SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len,
     const long long keys_o = static_cast<long long>(max_own) + (s.o_prefix ? prefix_len : 0);
     s.tiles_o = keys_o > 0 ? tiles(req_rows, kTileRows) : 0;
     s.tiles_p = prefix_items ? tiles(all_rows, kTileRows) : 0;
-    // Parts of about the same length: as many as two CTAs on every SM take at once, of 64 to
-    // 1024 keys (a shorter part is all latency, a longer one leaves SMs idle at the end).
-    // Half of max_own stands for the requests' mean.
+    // Parts of about the same length: as many as two CTAs on every SM take at once, of 64 keys
+    // (a shorter part is all latency) to 256 KB of K and V (the SMs finish within one part of each
+    // other). Half of max_own stands for the requests' mean.
     const long long units_o = static_cast<long long>(s.tiles_o) * n_kv * n_req, units_p = static_cast<long long>(s.tiles_p) * n_kv;
     const long long work = units_o * (s.o_prefix ? prefix_len + max_own / 2 : max_own / 2) + units_p * prefix_len;
     const long long part = std::min<long long>(1024, std::max<long long>(64, (work / 296 + 63) / 64 * 64));
@@ -530,13 +530,13 @@ void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, const Shar
 
 size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
                                  int hd) {
-    const SharedPlan s = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv);
+    const SharedPlan s = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd);
     const size_t units = s.direct() ? 0 : static_cast<size_t>(T) * n_heads * s.splits();
     return units * hd * sizeof(float) + units * sizeof(float2) + 512;
 }
 
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
-    const SharedPlan pl = plan_shared(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv);
+    const SharedPlan pl = plan_shared(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd);
     const size_t units = static_cast<size_t>(p.T) * p.n_heads * pl.splits();
     if (p.scratch_bytes < shared_attn_scratch_bytes(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd))
         throw ArgError("sdpa_shared_prefix: scratch too small");

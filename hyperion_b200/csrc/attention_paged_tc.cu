@@ -6,10 +6,10 @@
 // prefix and then its own keys (prefill). One pass over the keys with a running maximum:
 //   S = Q K^T (tcgen05.mma, fp32 in TMEM, two buffers), p = exp2(s - m) into a bf16 operand
 //   in shared memory, O += P V (fp32 in TMEM).
-// The reference maximum m of a row moves only when the running one has outgrown it by more
-// than 2^8: p then stays below 256, which costs neither bf16 nor the fp32 sums any
-// precision, and the 128 x head_dim accumulator is rescaled a few times per row instead of
-// once a block.
+// The reference m of a row (its first block's maximum) moves only when the running maximum
+// has outgrown it by more than 2^40. p and the sums have fp32's exponent range, so larger
+// values cost no precision (2^40 times 2^31 keys is far from overflow), and the 128 x head_dim
+// accumulator is next to never rescaled; a threshold of 2^8 rescaled in 12% of a warp's blocks.
 //
 // Warps 0..3 and 4..7: two softmax groups that take the blocks in turn, one row a thread, so
 //   that the exponentials of one block run under the loads, maxima and stores of the next (a
@@ -18,10 +18,11 @@
 // Warp 8: producer. Looks the pages up (32 table entries at a time, one a lane) and issues
 //   the tensor-map copies of the K and V blocks, one box a lane: 64 head_dim columns of
 //   min(page_size, 64) slots, 128-byte swizzled.
-// Warp 9: allocates TMEM and issues the MMAs from one lane, S(c + 1) before P V(c), so that
-//   the softmax of a block runs under the products of its neighbours. In the few blocks that
-//   stick out of the visible keys it first clears the V rows outside: what a pool holds there
-//   may be NaN, and 0 * NaN would reach the sums.
+// Warp 9: allocates TMEM and issues the MMAs from one lane, S(c + 2) before P V(c), so that
+//   the softmax of a block runs under the products of its neighbours.
+// In the few blocks that stick out of the visible keys the softmax group clears the V rows
+// outside before it hands P over: what a pool holds there may be NaN, and 0 * NaN would reach
+// the sums.
 // Every mbarrier wait is bounded; TMEM is freed before the CTA exits.
 #include "attention_paged.cuh"
 #include "tcgen05.cuh"
@@ -41,25 +42,24 @@ constexpr int kSoftWarps = 8;
 constexpr int kGroupWarps = 4;
 constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1;
 constexpr int kThreads = kSoftWarps * 32 + 64;
-constexpr float kLazy = 8.f;  // log2 of how far a row's maximum may outgrow its reference
+constexpr float kLazy = 40.f;  // log2 of how far a row's maximum may outgrow its reference
 
+// Shared memory: the ring of K and V blocks and two P blocks. The queries are in TMEM: as a
+// shared-memory operand they would be read again for every block (64 KB of 224 KB a block at
+// head_dim 256, where shared memory is what the kernel saturates).
 template <int HD>
 struct TcShared {
-    static constexpr uint32_t kTmemCols = HD > 128 ? 512 : 256;  // S 2 x 64 + O HD
+    static constexpr uint32_t kTmemCols = HD == 64 ? 256 : 512;  // S 2 x 64, O HD, Q HD / 2
     static constexpr int kSub = HD / 64;
-    static constexpr int kSlots = HD == 256 ? 4 : 8;
-    static constexpr int kPBufs = HD == 256 ? 1 : 2;  // a second one does not fit beside head_dim 256
-    static constexpr int kQBytes = kRows * HD * 2;
+    static constexpr int kSlots = HD == 256 ? 6 : 12;
     static constexpr int kTileBytes = kKeys * HD * 2;
     static constexpr int kPBytes = kRows * kKeys * 2;
-    static constexpr int kOffSlots = kQBytes;
-    static constexpr int kOffP = kOffSlots + kSlots * kTileBytes;
-    static constexpr int kOffRef = kOffP + kPBufs * kPBytes;  // float [kRows]: the rows' references
-    static constexpr int kOffSum = kOffRef + kRows * 4;       // float [kRows]: the second group's sums
-    static constexpr int kOffPos = kOffSum + kRows * 4;       // int [kRows]: positions
-    static constexpr int kOffRow = kOffPos + kRows * 4;       // int [kRows]: token * n_heads + head
-    static constexpr int kOffBars = kOffRow + kRows * 4;
-    static constexpr int kSmem = kOffBars + 256 + 1024;          // + alignment slack
+    static constexpr int kOffP = kSlots * kTileBytes;
+    static constexpr int kOffSum = kOffP;                    // float [kRows], once P is no longer read
+    static constexpr int kOffRef = kOffP + 2 * kPBytes;      // float [kRows]: the rows' references
+    static constexpr int kOffPos = kOffRef + kRows * 4;      // int [kRows]: positions
+    static constexpr int kOffBars = kOffPos + kRows * 4;
+    static constexpr int kSmem = kOffBars + 384 + 1024;      // + alignment slack
 };
 
 __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
@@ -87,17 +87,21 @@ __device__ __forceinline__ void wait_b(bool& ok, uint32_t bar, uint32_t parity) 
     ok = false;
 }
 
+// The same by a whole warp, which goes on as one.
+__device__ __forceinline__ void warp_wait(bool& ok, uint32_t bar, uint32_t parity) {
+    if (!ok || __all_sync(0xffffffffu, try_wait(bar, parity))) return;
+    const uint64_t t0 = now_ns();
+    do {
+        if (__all_sync(0xffffffffu, try_wait(bar, parity))) return;
+    } while (__all_sync(0xffffffffu, now_ns() - t0 < 500000000ull));
+    if ((threadIdx.x & 31) == 0) atomicAdd(&g_shared_attn_wait_timeouts, 1);
+    ok = false;
+}
+
 // Instruction descriptor: bf16 A and B, f32 D; B MN-major when b_mn.
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
            (static_cast<uint32_t>(M >> 4) << 24);
-}
-
-// MN-major 128-byte-swizzle descriptor: rows are keys, 64 head_dim values per 128-byte row;
-// 64-wide groups `lbo` bytes apart, 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t mn_desc(uint32_t smem_addr, uint32_t lbo) {
-    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
-           static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
 
 // Thread l writes TMEM lane (lane field of taddr) + l, 32 consecutive columns.
@@ -110,6 +114,35 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Descriptors are passed as their lower words (address, leading offset); the upper one says
+// 1024 bytes between 8-row groups, version 1 and the 128-byte swizzle.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// D[tmem] = A * B^T (+ D when accumulate), issued by the lane whose `leader` is set: A in TMEM
+// (16 bf16 of a row in 8 columns) ...
+__device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate,
+                                           uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n mov.b64 b, {%2, %6};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHi)
+        : "memory");
+}
+// ... or in shared memory.
+__device__ __forceinline__ void mma_smem_a(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate,
+                                           uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n mov.b64 a, {%1, %6};\n"
+        " mov.b64 b, {%2, %6};\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t bar, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+        "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -150,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     shared_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                           const SharedAttnParams p, const SharedPlan pl, SharedParts parts) {
     using S = TcShared<HD>;
-    constexpr int SUB = S::kSub, SLOTS = S::kSlots, PB = S::kPBufs;
+    constexpr int SUB = S::kSub, SLOTS = S::kSlots;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* sm = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
     const uint32_t sbase = smem_u32(sm);
@@ -165,10 +198,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     id /= p.n_kv;
     const bool per_request = pl.tc_per_request != 0;
     const int tile = per_request ? id % pl.tc_tiles : id, req = per_request ? id / pl.tc_tiles : 0;
-    int t0 = 0, n_tok = p.T;
+    int t0 = 0, n_tok = p.T, own = 0;
+    bool broken = false;
     if (per_request) {
-        t0 = min(max(p.row_start[req], 0), p.T);
-        n_tok = min(min(p.row_start[req + 1], p.T) - t0, p.max_q);
+        const int first = p.row_start[req], next = p.row_start[req + 1], len = p.own_lens[req];
+        const long long most = min(static_cast<long long>(p.max_own), static_cast<long long>(p.max_blocks) * p.page_size);
+        t0 = min(max(first, 0), p.T);
+        n_tok = min(min(next, p.T) - t0, p.max_q);
+        own = static_cast<int>(min(static_cast<long long>(max(0, len)), most));
+        broken = len > most;  // with several parts the merge says so
     }
     const long long m0 = static_cast<long long>(tile) * kRows;
     const int rows = static_cast<int>(max(0ll, min(static_cast<long long>(kRows), static_cast<long long>(n_tok) * G - m0)));
@@ -177,7 +215,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (rows <= 0) return;
 
     int* s_pos = reinterpret_cast<int*>(sm + S::kOffPos);
-    int* s_row = reinterpret_cast<int*>(sm + S::kOffRow);
     float* s_ref = reinterpret_cast<float*>(sm + S::kOffRef);
     float* s_sum = reinterpret_cast<float*>(sm + S::kOffSum);
     const uint32_t slot_full = sbase + S::kOffBars;
@@ -190,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t q_full = o_full + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + S::kOffBars + 8 * (2 * SLOTS + 10));
     volatile int* s_bad = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert(8 * (2 * SLOTS + 10) + 8 <= 256, "barriers fit");
+    static_assert(8 * (2 * SLOTS + 10) + 8 <= 384, "barriers fit");
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
@@ -214,16 +251,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(smem_u32(tmem_slot), S::kTmemCols);
         tmem_relinquish();
     }
-    if (threadIdx.x < kRows) {
-        const int pr = static_cast<int>(m0) + min(static_cast<int>(threadIdx.x), rows - 1), tok = pr / G;
-        s_pos[threadIdx.x] = static_cast<int>(threadIdx.x) < rows ? p.row_pos[t0 + tok] : -1;
-        s_row[threadIdx.x] = (t0 + tok) * p.n_heads + hk * G + (pr - tok * G);
+    // softmax threads: row r of the tile is (token, head) pair m0 + r; its place, position and
+    // share of the query row (the groups take 64 elements in turn), on their way before the barrier
+    const int quad = warp & 3, group = warp >> 2, r = 32 * quad + lane;
+    constexpr int kQ = HD == 256 ? 2 : 1;
+    uint32_t qw[kQ][32];
+    int row = 0, pos = -1;
+    if (warp < kSoftWarps) {
+        const int pr = static_cast<int>(m0) + min(r, rows - 1), tok = pr / G;
+        row = (t0 + tok) * p.n_heads + hk * G + (pr - tok * G);
+        if (r < rows) pos = p.row_pos[t0 + tok];
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<size_t>(row) * HD);
+#pragma unroll
+        for (int j = 0; j < kQ; ++j)
+            if (HD > 64 || group == 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 v = r < rows ? src[8 * (2 * j + (HD > 64 ? group : 0)) + i] : make_uint4(0, 0, 0, 0);
+                    qw[j][4 * i] = v.x;
+                    qw[j][4 * i + 1] = v.y;
+                    qw[j][4 * i + 2] = v.z;
+                    qw[j][4 * i + 3] = v.w;
+                }
+            }
+        if (group == 0) s_pos[r] = pos;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t tmem_s = tmem, tmem_o = tmem + 128;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const uint32_t tmem_s = tmem, tmem_o = tmem + 128, tmem_q = tmem_o + HD;
 
     int pmin = INT_MAX, pmax = -1;
     for (int i = lane; i < kRows; i += 32)
@@ -235,16 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     pmax = __reduce_max_sync(0xffffffffu, pmax);
     const Segment sp = segment(p.prefix_table, 0, p.prefix_len, pmin, pmax, p.window);
     Segment so = {nullptr, p.prefix_len, 0, 0, 0};
-    bool broken = false;
-    if (per_request) {
-        const long long most = min(static_cast<long long>(p.max_own), static_cast<long long>(p.max_blocks) * p.page_size);
-        const int own = static_cast<int>(min(static_cast<long long>(max(0, p.own_lens[req])), most));
-        broken = p.own_lens[req] > most;  // with several parts the merge says so
-        so = segment(p.table + static_cast<size_t>(req) * p.max_blocks, p.prefix_len, own, pmin, pmax, p.window);
-    }
+    if (per_request) so = segment(p.table + static_cast<size_t>(req) * p.max_blocks, p.prefix_len, own, pmin, pmax, p.window);
     const int all = sp.blocks + so.blocks;
     const int c0 = static_cast<int>(static_cast<long long>(all) * split / pl.tc_splits);
-    const int nb = static_cast<int>(static_cast<long long>(all) * (split + 1) / pl.tc_splits) - c0;
+    const int nb = __shfl_sync(0xffffffffu, static_cast<int>(static_cast<long long>(all) * (split + 1) / pl.tc_splits) - c0, 0);
     // the segment and first key of this part's block c
     auto block = [&](int c, int& key0) -> const Segment& {
         const int b = c0 + c;
@@ -254,124 +305,130 @@ __global__ void __launch_bounds__(kThreads, 1)
         return s;
     };
     bool ok = true;
+    // The ring's items in the order of the products: K 0, K 1, V 0, K 2, V 1, .., K nb-1, V nb-2, V nb-1:
+    // K c is item 2 c - 1 (0 for c = 0), V c is item 2 c + 2 (2 nb - 1 for the last).
 
     if (warp == kTmaWarp) {
         const int piece = min(p.page_size, kKeys);  // slots of one box
         const int pieces = kKeys / piece, boxes = SUB * pieces;
         const int per_load = pieces == 1 ? 32 : 32 / pieces;  // blocks whose pages 32 lanes hold
-        int page = 0;
-        for (int c = 0; c < nb; ++c) {
-            int key0;
-            if (c % per_load == 0) {
-                // lane i: the page of piece i % pieces of block c + i / pieces; -1 past the visible keys
-                page = -1;
-                if (c + lane / pieces < nb) {
-                    const Segment& s = block(c + lane / pieces, key0);
-                    const int key = key0 + (lane % pieces) * piece;
-                    if (key < s.hi && key + piece > s.lo) {
-                        page = s.table[key / p.page_size];
-                        if (page < 0 || page >= p.n_pages) {
-                            *s_bad = 1;
-                            page = -1;
-                        }
-                    }
+        int page_k = -1, page_v = -1;
+        // lane i: the table's entry for piece i % pieces of block c + i / pieces; -1 past the visible keys
+        auto look_up = [&](int c) {
+            int page = -1, key0;
+            if (c + lane / pieces < nb) {
+                const Segment& s = block(c + lane / pieces, key0);
+                const int key = key0 + (lane % pieces) * piece;
+                if (key < s.hi && key + piece > s.lo) {
+                    page = s.table[key / p.page_size];
+                    if (page < 0) page = INT_MAX;  // told from "not needed"
                 }
             }
+            return page;
+        };
+        int page_n = look_up(0);  // loaded one batch ahead of its use
+        auto copy = [&](int i, int c, int page, const CUtensorMap* map) {
+            int key0;
             block(c, key0);
-            const int src = (c % per_load) * pieces;
-            const int mine = __shfl_sync(0xffffffffu, page, src + lane % pieces);
+            const int mine = __shfl_sync(0xffffffffu, page, (c % per_load) * pieces + lane % pieces);
             // a page that nobody sees (or none): a box past the pool, which reads as zeros
             const int at = mine >= 0 ? mine * p.page_size + (key0 + (lane % pieces) * piece) % p.page_size : p.n_pages * p.page_size;
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                const int i = 2 * c + kv, slot = i % SLOTS;
-                if (i >= SLOTS) wait_b(ok, slot_empty + 8 * slot, ((i / SLOTS) - 1) & 1);
-                if (lane == 0) mbar_expect_tx(slot_full + 8 * slot, S::kTileBytes);
-                __syncwarp();
-                if (lane < boxes) {
-                    const int d = lane / pieces;
-                    tma_load_3d(sbase + S::kOffSlots + slot * S::kTileBytes + d * (kKeys * 128) + (lane % pieces) * piece * 128,
-                                kv ? &tm_v : &tm_k, 64 * d, hk, at, slot_full + 8 * slot);
-                }
+            const int slot = i % SLOTS;
+            if (i >= SLOTS) wait_b(ok, slot_empty + 8 * slot, ((i / SLOTS) - 1) & 1);
+            if (lane == 0) mbar_expect_tx(slot_full + 8 * slot, S::kTileBytes);
+            __syncwarp();
+            if (lane < boxes) {
+                const int d = lane / pieces;
+                tma_load_3d(sbase + slot * S::kTileBytes + d * (kKeys * 128) + (lane % pieces) * piece * 128, map,
+                            64 * d, hk, at, slot_full + 8 * slot);
             }
+        };
+        // in the order of the products: K 0, K 1, V 0, K 2, V 1, ...
+        for (int c = 0; c < nb + 1; ++c) {
+            if (c < nb) {
+                if (c % per_load == 0) {
+                    page_v = page_k;  // of the blocks before: the last V is still to come
+                    page_k = page_n;
+                    page_n = look_up(c + per_load);
+                    if (page_k >= p.n_pages) {
+                        *s_bad = 1;
+                        page_k = -1;
+                    }
+                }
+                copy(c == 0 ? 0 : 2 * c - 1, c, page_k, &tm_k);
+            }
+            if (c >= 1) copy(c < nb ? 2 * c : 2 * nb - 1, c - 1, (c - 1) / per_load == c / per_load || c == nb ? page_k : page_v, &tm_v);
         }
     } else if (warp == kMmaWarp) {
+        // The whole warp runs the loop with warp-uniform values and lane 0 alone issues, by a
+        // predicate: descriptors then stay in uniform registers. With the issue in a one-lane branch
+        // an MMA took some 65 cycles to issue, twice what the tensor cores need for it.
         constexpr uint32_t id_s = idesc_bf16(kRows, kKeys, false);
         constexpr uint32_t id_o = idesc_bf16(kRows, HD, true);
-        auto issue_s = [&](int c) {
-            const int i = 2 * c, slot = i % SLOTS, sb = c & 1;
-            wait_b(ok, slot_full + 8 * slot, (i / SLOTS) & 1);
-            if (c >= 2) wait_b(ok, s_empty + 8 * sb, ((c >> 1) - 1) & 1);
+        const uint32_t leader = lane == 0;
+        const uint32_t ring = sbase >> 4, p_lo = ((sbase + S::kOffP) >> 4) | (1u << 16);
+        auto issue_s = [&](int sb, int slot) {
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t kbase = sbase + S::kOffSlots + slot * S::kTileBytes;
+            const uint32_t lo = (ring + slot * (S::kTileBytes >> 4)) | (1u << 16);
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint64_t ad = sw128_kmajor_desc(sbase + (kk >> 2) * (kRows * 128)) + 2 * (kk & 3);
-                    const uint64_t bd = sw128_kmajor_desc(kbase + (kk >> 2) * (kKeys * 128)) + 2 * (kk & 3);
-                    tc_mma_f16(tmem_s + 64 * sb, ad, bd, id_s, kk > 0 ? 1u : 0u);
-                }
-                tc_commit(s_full + 8 * sb);
-                tc_commit(slot_empty + 8 * slot);
-            }
-            __syncwarp();
-        };
-        auto issue_pv = [&](int c) {
-            const int i = 2 * c + 1, slot = i % SLOTS, pb = c % PB;
-            wait_b(ok, slot_full + 8 * slot, (i / SLOTS) & 1);
-            int key0;
-            const Segment& s = block(c, key0);
-            if (key0 < s.lo || key0 + kKeys > s.hi) {
-                unsigned char* vt = sm + S::kOffSlots + slot * S::kTileBytes;
-                const int head = min(kKeys, max(0, s.lo - key0)), tail = min(kKeys, s.hi - key0);  // rows before, from
-                for (int j = lane; j < (head + kKeys - tail) * SUB * 8; j += 32) {
-                    const int n = j / (SUB * 8), key = n < head ? n : tail + n - head, ch = j % (SUB * 8);
-                    *reinterpret_cast<uint4*>(vt + (ch >> 3) * (kKeys * 128) + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async();
-                __syncwarp();
-            }
-            wait_b(ok, p_full + 8 * (c & 1), (c >> 1) & 1);
-            tc_fence_after();
-            if (lane == 0) {
-                const uint32_t vbase = sbase + S::kOffSlots + slot * S::kTileBytes;
-#pragma unroll
-                for (int kk = 0; kk < kKeys / 16; ++kk) {
-                    const uint64_t ad = sw128_kmajor_desc(sbase + S::kOffP + pb * S::kPBytes) + 2 * kk;
-                    const uint64_t bd = mn_desc(vbase + kk * 2048, kKeys * 128);
-                    tc_mma_f16(tmem_o, ad, bd, id_o, (c > 0 || kk > 0) ? 1u : 0u);
-                }
-                tc_commit(pv_done + 8 * (c & 1));
-                tc_commit(slot_empty + 8 * slot);
-            }
-            __syncwarp();
+            for (int kk = 0; kk < HD / 16; ++kk)
+                mma_tmem_a(tmem_s + 64 * sb, tmem_q + 8 * kk, lo + (kk >> 2) * (kKeys * 128 >> 4) + 2 * (kk & 3), id_s, kk > 0, leader);
+            commit_if(s_full + 8 * sb, leader);
+            commit_if(slot_empty + 8 * slot, leader);
         };
         if (nb > 0) {
-            wait_b(ok, q_full, 0);
-            issue_s(0);
-            for (int c = 0; c < nb; ++c) {
-                if (c + 1 < nb) issue_s(c + 1);
-                issue_pv(c);
+            warp_wait(ok, q_full, 0);
+            warp_wait(ok, slot_full, 0);
+            issue_s(0, 0);
+            int ks = 1, kph = 0, vs = nb > 1 ? 2 : 1, vph = 0;  // ring places of the next K and V, their phases
+            if (nb > 1) {
+                warp_wait(ok, slot_full + 8 * ks, kph);
+                issue_s(1, ks);
             }
-            if (lane == 0) tc_commit(o_full);
+            // S(c + 2) goes before P V(c): its buffer is free as soon as the softmax of block c has
+            // read it, and the group finds it ready when it is through with block c
+            for (int c = 0; c < nb; ++c) {
+                const int sb = c & 1;
+                const bool v_here = try_wait(slot_full + 8 * vs, vph);  // asked for ahead of its use
+                if (c + 2 < nb) {
+                    ks += 2;
+                    if (ks >= SLOTS) {
+                        ks -= SLOTS;
+                        kph ^= 1;
+                    }
+                    const bool k_here = try_wait(slot_full + 8 * ks, kph);
+                    warp_wait(ok, s_empty + 8 * sb, (c >> 1) & 1);
+                    if (!__all_sync(0xffffffffu, k_here)) warp_wait(ok, slot_full + 8 * ks, kph);
+                    issue_s(sb, ks);
+                }
+                if (!__all_sync(0xffffffffu, v_here)) warp_wait(ok, slot_full + 8 * vs, vph);
+                warp_wait(ok, p_full + 8 * sb, (c >> 1) & 1);
+                tc_fence_after();
+                const uint32_t vlo = (ring + vs * (S::kTileBytes >> 4)) | (((kKeys * 128 >> 4) & 0x3FFFu) << 16);
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                    mma_smem_a(tmem_o, p_lo + sb * (S::kPBytes >> 4) + 2 * kk, vlo + kk * (2048 >> 4), id_o, c > 0 || kk > 0, leader);
+                commit_if(pv_done + 8 * sb, leader);
+                commit_if(slot_empty + 8 * vs, leader);
+                vs += c + 2 < nb ? 2 : 1;
+                if (vs >= SLOTS) {
+                    vs -= SLOTS;
+                    vph ^= 1;
+                }
+            }
+            commit_if(o_full, leader);
         }
     } else {
-        // queries: row r of the tile, 16-byte chunk ch, in the K-major swizzled layout
-#pragma unroll 8
-        for (int i = threadIdx.x; i < kRows * (HD / 8); i += kSoftWarps * 32) {
-            const int r = i / (HD / 8), ch = i % (HD / 8);
-            const uint4 v = r < rows ? *reinterpret_cast<const uint4*>(p.q + static_cast<size_t>(s_row[r]) * HD + 8 * ch)
-                                     : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(sm + (ch >> 3) * (kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+        const uint32_t lane_off = static_cast<uint32_t>(32 * quad) << 16;
+        // queries into TMEM: lane r, two bf16 a column
+        if (HD > 64 || group == 0) {
+#pragma unroll
+            for (int j = 0; j < kQ; ++j) tmem_st_32x32b_x32(tmem_q + lane_off + 32 * (2 * j + (HD > 64 ? group : 0)), qw[j]);
+            tmem_st_wait();
         }
-        fence_proxy_async();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
-
-        const int quad = warp & 3, group = warp >> 2;
-        const int r = 32 * quad + lane;
-        const int pos = s_pos[r];
-        const uint32_t lane_off = static_cast<uint32_t>(32 * quad) << 16;
         const int mine = 1 + 2 * quad + group, other = 1 + 2 * quad + (group ^ 1);  // hand-over barriers
         // with a plain positive scale the maximum is taken over the raw products
         const bool plain = p.softcap <= 0.f && p.scale > 0.f;
@@ -379,7 +436,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY;  // the reference that l is held at
         float l = 0.f;
         for (int c = group; c < nb; c += 2) {
-            const int pb = c % PB;
             int key0;
             const Segment& s = block(c, key0);
             wait_b(ok, s_full + 8 * group, (c >> 1) & 1);
@@ -426,13 +482,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 s_ref[r] = now;
                 hand_on(mine);
             }
-            // P V(c - 2) used this group's barrier last; the next use is P V(c), which needs this
-            // group's P(c), so the barrier is one phase ahead at most and the parity is enough. With
-            // P V(c - 2) done the same holds for the other group's barrier and P V(c - 1).
-            if (c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);
             if (c > 0 && __any_sync(0xffffffffu, move)) {
                 const float f = move ? shared_ex2(ref - now) : 1.f;
-                wait_b(ok, pv_done + 8 * (group ^ 1), ((c - 1) >> 1) & 1);  // P V(c - 1) is done
+                // P V(c - 1) is done. Its barrier's phase is told by parity: with P V(c - 2) done it is
+                // at most one phase behind, and P V(c + 1), the next use, cannot be through before
+                // P V(c), which needs this group's P(c).
+                if (c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);
+                wait_b(ok, pv_done + 8 * (group ^ 1), ((c - 1) >> 1) & 1);
                 tc_fence_after();
 #pragma unroll 1
                 for (int col = 0; col < HD; col += 32) {
@@ -460,20 +516,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sum[(2 * i + 1) & 3] += __uint_as_float(w[i] & 0xffff0000u);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if (PB == 1 && c > 0) wait_b(ok, pv_done + 8 * (group ^ 1), ((c - 1) >> 1) & 1);  // the only buffer
-            unsigned char* prow = sm + S::kOffP + pb * S::kPBytes + r * 128;
+            if (c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);  // the buffer's last reader
+            unsigned char* prow = sm + S::kOffP + group * S::kPBytes + r * 128;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 *reinterpret_cast<uint4*>(prow + ((i ^ (r & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            if (key0 < s.lo || key0 + kKeys > s.hi) {
+                // V rows that no row of the tile sees; the block's V has its place in the ring to
+                // itself until P V(c), and what held the place before was used up by a product
+                // issued ahead of S(c)
+                const int i = c + 1 < nb ? 2 * c + 2 : 2 * nb - 1, slot = i % SLOTS;
+                wait_b(ok, slot_full + 8 * slot, (i / SLOTS) & 1);
+                unsigned char* vt = sm + slot * S::kTileBytes;
+                const int head = min(kKeys, max(0, s.lo - key0)), tail = min(kKeys, s.hi - key0);  // rows before, from
+                for (int j = r; j < (head + kKeys - tail) * SUB * 8; j += kRows) {
+                    const int n = j / (SUB * 8), key = n < head ? n : tail + n - head, ch = j % (SUB * 8);
+                    *reinterpret_cast<uint4*>(vt + (ch >> 3) * (kKeys * 128) + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+            }
             fence_proxy_async();  // generic-proxy writes -> the MMA's async-proxy reads
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + 8 * group);
         }
         // ---- the row's sum over both groups at the last reference, then its accumulator: the
         // group that took the last block holds that reference
+        if (nb > 0) {
+            wait_b(ok, o_full, 0);
+            tc_fence_after();
+        }
         const int last = nb > 0 ? (nb - 1) & 1 : 0;
         if (group != last) {
-            s_sum[r] = l;
+            s_sum[r] = l;  // where P was: every product is done
             s_ref[r] = m;  // what it handed on last, if anything
             hand_on(9 + quad);
         } else {
@@ -481,18 +554,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float om = s_ref[r], z = m == -INFINITY ? 0.f : m;
             l += s_sum[r] * shared_ex2(om - z);
         }
-        if (nb > 0) {
-            wait_b(ok, o_full, 0);
-            tc_fence_after();
-        }
         if (*s_bad || (broken && parts.direct)) {
             m = 0.f;
             l = __int_as_float(0x7fffffff);
         }
         if (!parts.direct) {
-            if (group == last && r < rows) parts.ml[static_cast<size_t>(s_row[r]) * parts.n + split] = make_float2(m, l);
+            if (group == last && r < rows) parts.ml[static_cast<size_t>(row) * parts.n + split] = make_float2(m, l);
             if (nb > 0) {
-                float* dst = parts.o + (static_cast<size_t>(s_row[r]) * parts.n + split) * HD;
+                float* dst = parts.o + (static_cast<size_t>(row) * parts.n + split) * HD;
 #pragma unroll 1
                 for (int col = group * (HD / 2); col < (group + 1) * (HD / 2); col += 32) {
                     uint32_t o[32];
@@ -510,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("bar.sync 13, 256;" ::: "memory");  // the softmax warps
             l = s_sum[r];
             const float inv = l > 0.f ? 1.0f / l : l;  // no key seen: 0 (nothing was accumulated); NaN stays
-            uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(s_row[r]) * HD);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(row) * HD);
 #pragma unroll 1
             for (int col = group * (HD / 2); col < (group + 1) * (HD / 2); col += 32) {
                 uint32_t o[32];

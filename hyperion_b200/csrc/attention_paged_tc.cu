@@ -15,10 +15,10 @@
 //   that the exponentials of one block run under the loads, maxima and stores of the next (a
 //   single group leaves its own latency, some 3000 cycles a block, in the chain). A group
 //   hands the rows' references on to the other before it starts its exponentials.
-// Warp 8: producer. Looks the pages up (32 table entries at a time, one a lane) and issues
-//   the tensor-map copies of the K and V blocks, one box a lane: 64 head_dim columns of
-//   min(page_size, 64) slots, 128-byte swizzled.
-// Warp 9: allocates TMEM and issues the MMAs from one lane, S(c + 2) before P V(c), so that
+// Warps 8 and 9: producers of the K and of the V blocks. They look the pages up (32 table
+//   entries at a time, one a lane, a batch ahead) and issue the tensor-map copies: boxes of 64
+//   head_dim columns of min(page_size, 64) slots, 128-byte swizzled.
+// Warp 10: allocates TMEM and issues the MMAs from one lane, S(c + 2) before P V(c), so that
 //   the softmax of a block runs under the products of its neighbours.
 // In the few blocks that stick out of the visible keys the softmax group clears the V rows
 // outside before it hands P over: what a pool holds there may be NaN, and 0 * NaN would reach
@@ -40,8 +40,8 @@ constexpr int kRows = kTcRows;  // 128
 constexpr int kKeys = 64;
 constexpr int kSoftWarps = 8;
 constexpr int kGroupWarps = 4;
-constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1;
-constexpr int kThreads = kSoftWarps * 32 + 64;
+constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 2;  // two producers: K, V
+constexpr int kThreads = kSoftWarps * 32 + 96;
 constexpr float kLazy = 40.f;  // log2 of how far a row's maximum may outgrow its reference
 
 // Shared memory: the ring of K and V blocks and two P blocks. The queries are in TMEM: as a
@@ -136,6 +136,15 @@ __device__ __forceinline__ void mma_smem_a(uint32_t d_tmem, uint32_t a_lo, uint3
         "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n mov.b64 a, {%1, %6};\n"
         " mov.b64 b, {%2, %6};\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d_tmem),
         "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHi)
+        : "memory");
+}
+// Issued by the lane whose `leader` is set, of a warp that goes on as one: a copy issued lane by
+// lane with lane-dependent coordinates takes over 100 cycles.
+__device__ __forceinline__ void tma_load_if(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %6, 0;\n"
+        " @q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void commit_if(uint32_t bar, uint32_t leader) {
@@ -305,59 +314,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         return s;
     };
     bool ok = true;
-    // The ring's items in the order of the products: K 0, K 1, V 0, K 2, V 1, .., K nb-1, V nb-2, V nb-1:
-    // K c is item 2 c - 1 (0 for c = 0), V c is item 2 c + 2 (2 nb - 1 for the last).
-
-    if (warp == kTmaWarp) {
-        const int piece = min(p.page_size, kKeys);  // slots of one box
-        const int pieces = kKeys / piece, boxes = SUB * pieces;
+    if (warp == kTmaWarp || warp == kTmaWarp + 1) {
+        const bool is_v = warp != kTmaWarp;
+        const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+        const int piece = min(p.page_size, kKeys), shift = __ffs(piece) - 1;  // slots of one box
+        const int pieces = kKeys >> shift, in_page = p.page_size - 1;
         const int per_load = pieces == 1 ? 32 : 32 / pieces;  // blocks whose pages 32 lanes hold
-        int page_k = -1, page_v = -1;
-        // lane i: the table's entry for piece i % pieces of block c + i / pieces; -1 past the visible keys
-        auto look_up = [&](int c) {
-            int page = -1, key0;
-            if (c + lane / pieces < nb) {
-                const Segment& s = block(c + lane / pieces, key0);
-                const int key = key0 + (lane % pieces) * piece;
-                if (key < s.hi && key + piece > s.lo) {
-                    page = s.table[key / p.page_size];
-                    if (page < 0) page = INT_MAX;  // told from "not needed"
-                }
-            }
-            return page;
+        const int page_shift = __ffs(p.page_size) - 1;
+        const uint32_t leader = lane == 0;
+        // lane i: piece i % pieces of block c + i / pieces; whether some row sees a key of it
+        auto piece_of = [&](int c, int& key, const int*& table) {
+            c += lane / pieces;
+            if (c >= nb) return false;
+            const Segment& s = block(c, key);
+            key += (lane % pieces) << shift;
+            table = s.table;
+            return key < s.hi && key + piece > s.lo;
         };
-        int page_n = look_up(0);  // loaded one batch ahead of its use
-        auto copy = [&](int i, int c, int page, const CUtensorMap* map) {
-            int key0;
-            block(c, key0);
-            const int mine = __shfl_sync(0xffffffffu, page, (c % per_load) * pieces + lane % pieces);
-            // a page that nobody sees (or none): a box past the pool, which reads as zeros
-            const int at = mine >= 0 ? mine * p.page_size + (key0 + (lane % pieces) * piece) % p.page_size : p.n_pages * p.page_size;
-            const int slot = i % SLOTS;
-            if (i >= SLOTS) wait_b(ok, slot_empty + 8 * slot, ((i / SLOTS) - 1) & 1);
+        auto look_up = [&](int c) {
+            int key;
+            const int* table;
+            return piece_of(c, key, table) ? table[key >> page_shift] : 0;
+        };
+        int next = look_up(0), at = 0;  // the pages one batch ahead of their use; lane i's first slot
+        for (int c = 0; c < nb; ++c) {
+            if (c % per_load == 0) {
+                int key;
+                const int* table;
+                const bool seen = piece_of(c, key, table), there = next >= 0 && next < p.n_pages;
+                if (seen && !there) *s_bad = 1;
+                // pieces that nobody sees (and bad pages): a box past the pool, which reads as zeros
+                at = seen && there ? (next << page_shift) + (key & in_page) : p.n_pages << page_shift;
+                next = look_up(c + per_load);
+            }
+            // the ring's items in the order of the products: K 0, K 1, V 0, K 2, V 1, .., K nb-1, V nb-2, V nb-1
+            const int i = is_v ? (c + 1 < nb ? 2 * c + 2 : 2 * nb - 1) : (c == 0 ? 0 : 2 * c - 1), slot = i % SLOTS;
+            if (i >= SLOTS) warp_wait(ok, slot_empty + 8 * slot, ((i / SLOTS) - 1) & 1);
             if (lane == 0) mbar_expect_tx(slot_full + 8 * slot, S::kTileBytes);
             __syncwarp();
-            if (lane < boxes) {
-                const int d = lane / pieces;
-                tma_load_3d(sbase + slot * S::kTileBytes + d * (kKeys * 128) + (lane % pieces) * piece * 128, map,
-                            64 * d, hk, at, slot_full + 8 * slot);
+            const uint32_t dst = sbase + slot * S::kTileBytes;
+            for (int q = 0; q < pieces; ++q) {
+                const int row = __shfl_sync(0xffffffffu, at, (c % per_load) * pieces + q);
+#pragma unroll
+                for (int d = 0; d < SUB; ++d)
+                    tma_load_if(dst + d * (kKeys * 128) + ((q << shift) << 7), map, 64 * d, hk, row, slot_full + 8 * slot, leader);
             }
-        };
-        // in the order of the products: K 0, K 1, V 0, K 2, V 1, ...
-        for (int c = 0; c < nb + 1; ++c) {
-            if (c < nb) {
-                if (c % per_load == 0) {
-                    page_v = page_k;  // of the blocks before: the last V is still to come
-                    page_k = page_n;
-                    page_n = look_up(c + per_load);
-                    if (page_k >= p.n_pages) {
-                        *s_bad = 1;
-                        page_k = -1;
-                    }
-                }
-                copy(c == 0 ? 0 : 2 * c - 1, c, page_k, &tm_k);
-            }
-            if (c >= 1) copy(c < nb ? 2 * c : 2 * nb - 1, c - 1, (c - 1) / per_load == c / per_load || c == nb ? page_k : page_v, &tm_v);
         }
     } else if (warp == kMmaWarp) {
         // The whole warp runs the loop with warp-uniform values and lane 0 alone issues, by a

@@ -22,6 +22,8 @@
 
 namespace hyb {
 
+__device__ int g_shared_small_wait_timeouts = 0;
+
 namespace {
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
@@ -36,16 +38,6 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& a, uint32_t& 
                  : "r"(addr)
                  : "memory");
 }
-// 16 bytes global -> shared, or 16 zero bytes (nothing is read) when !take.
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 constexpr int kTileRows = 16;
 constexpr int kWarps = 4;
 constexpr int kSlice = 16;  // keys of one warp step
@@ -113,34 +105,45 @@ __device__ __forceinline__ Keys keys_of(const int* table, int base, int len, int
 
 template <int HD>
 struct SmallPlan {
-    // K or V of one slice is one stage; 24 KB a warp (12 KB for head_dim 64), so that two CTAs
-    // (four) share an SM and one streams while the other starts or ends
+    // K or V of one slice is one stage, head_dim / 64 boxes of [16 keys][128 bytes]; 24 KB a warp,
+    // so that two CTAs share an SM and one streams while the other starts or ends
     static constexpr int kHalf = kSlice * HD * 2;
-    static constexpr int kStages = HD == 256 ? 3 : 6;
+    static constexpr int kStages = 24 * 1024 / kHalf;
     static constexpr int kRing = kWarps * kStages * kHalf;
     static constexpr int kMerge = kWarps * kTileRows * HD * 4;
-    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+    static constexpr int kBars = kRing > kMerge ? kRing : kMerge;
+    static constexpr int kSmem = kBars + kWarps * kStages * 8 + 1024;  // + alignment slack
 };
 
 // One CTA: up to 16 rows (row m of a tile = token m / G, head m % G of the KV head's group)
 // against one part of the prefix, or of one request's keys. Each warp takes every fourth
-// 16-key slice of the part on its own: cp.async into its own ring (zero fill of keys that no
-// row of the tile sees, so whatever the pool holds there cannot reach a product), QK^T and PV
-// on mma.sync m16n8k16, online softmax; the four warps' results are joined at the end. Rows
+// 16-key slice of the part on its own: tensor-map copies into its own ring, QK^T and PV on
+// mma.sync m16n8k16, online softmax; the four warps' results are joined at the end. V rows
+// of keys that no row of the tile sees are cleared before the product (0 * NaN). Rows
 // share every byte of K and V that is loaded, so up to 16 rows cost the same traffic as one:
-// HBM bound. The chain in front of the first copy is three loads deep: lengths, row starts
-// and pages; positions; keys.
+// HBM bound, if the eight warps of an SM get through a slice in 1.5 us at head_dim 128; so
+// copies are issued for a whole slice at once (per-lane 16-byte copies took half of 660
+// instructions a slice), and masks and rescaling sit behind warp-uniform branches.
+// The chain in front of the first copy is three loads deep: lengths, row starts and pages;
+// positions; keys.
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32, 2) shared_attn_small_kernel(const SharedAttnParams p, const SharedPlan pl,
-                                                                           SharedParts parts, int after_tc) {
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    shared_attn_small_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                             const SharedAttnParams p, const SharedPlan pl, SharedParts parts, int after_tc) {
     using SP = SmallPlan<HD>;
-    constexpr int KS = HD / 16, CH = HD / 8, ST = SP::kStages;
-    extern __shared__ __align__(128) unsigned char sm[];
+    constexpr int KS = HD / 16, SUB = HD / 64, ST = SP::kStages;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* sm = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
     __shared__ float s_m[kWarps][kTileRows], s_l[kWarps][kTileRows];
     __shared__ int s_row[kTileRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.n_heads / p.n_kv;
+    const uint32_t leader = lane == 0;
+    const uint32_t ring = smem_u32(sm) + warp * ST * SP::kHalf, full = smem_u32(sm) + SP::kBars + warp * ST * 8;
     pdl_launch_dependents();
+    if (lane < ST) mbar_init(full + 8 * lane, 1);
+    mbar_init_fence();
+    __syncwarp();
 
     // ---- which part
     int id = blockIdx.x;
@@ -231,87 +234,83 @@ __global__ void __launch_bounds__(kWarps * 32, 2) shared_attn_small_kernel(const
     float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
     bool bad = false;
 
-    const uint32_t ring = smem_u32(sm) + warp * ST * SP::kHalf;
-    auto load_pages = [&](int from) {  // of this warp's slices from .. from + 31
+    bool ok = true;
+    const int page_shift = __ffs(p.page_size) - 1, in_page = p.page_size - 1;
+    auto load_pages = [&](int from) {  // of this warp's slices from .. from + 31, as first slots
         const int i = from + lane, s = s0 + warp + i * kWarps;
-        if (from > 0 || p.window > 0) {
-            pages = 0;
-            if (i < mine) {
-                const bool a = s < ka.slices;
-                pages = (a ? ka.table : kb.table)[(a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice) / p.page_size];
-            }
-        }
-        if (i < mine && (pages < 0 || pages >= p.n_pages)) {
-            bad = true;
-            pages = -1;
-        }
+        const bool a = s < ka.slices;
+        const int key = a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
+        if ((from > 0 || p.window > 0) && i < mine) pages = (a ? ka.table : kb.table)[key >> page_shift];
+        const bool there = pages >= 0 && pages < p.n_pages;
+        if (i < mine && !there) bad = true;
+        // slices without a visible key, and bad pages: a box past the pool, which reads as zeros
+        pages = i < mine && there && key < (a ? ka.hi : kb.hi) ? (pages << page_shift) + (key & in_page) : p.n_pages << page_shift;
     };
     int f_slot = 0;
     auto fetch = [&](int j) {  // K (even) or V (odd) of this warp's slice j / 2
         const int i = j >> 1;
         if (i < mine) {
             if ((j & 63) == 0) load_pages(i);
-            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-            const int s = s0 + warp + i * kWarps;
-            const bool a = s < ka.slices;
-            const int key0 = a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
-            const int lo = a ? ka.lo : kb.lo, hi = a ? ka.hi : kb.hi;
-            const size_t cell = (static_cast<size_t>(max(page, 0)) * p.page_size + key0 % p.page_size) * p.n_kv + hk;
-            const bf16* src = ((j & 1) ? p.v_pool : p.k_pool) + cell * HD;
-            const uint32_t dst = ring + f_slot * SP::kHalf;
-            const size_t row = static_cast<size_t>(p.n_kv) * HD;
-            constexpr int KPI = 32 / CH > 0 ? 32 / CH : 1;  // keys of one instruction
-            const int k_lane = lane / CH, ch = lane % CH;
-            const int from = lo - key0, to = page >= 0 ? hi - key0 : 0;
-            src += k_lane * row + ch * 8;
+            const int at = __shfl_sync(0xffffffffu, pages, i & 31);
+            const uint32_t bar = full + 8 * f_slot, dst = ring + f_slot * SP::kHalf;
+            if (lane == 0) mbar_expect_tx(bar, SP::kHalf);
+            __syncwarp();
 #pragma unroll
-            for (int q = 0; q < kSlice / KPI; ++q) {
-                const int key = q * KPI + k_lane;
-                cp16(dst + key * (HD * 2) + ((ch ^ (key & 7)) << 4), src + q * KPI * row, key >= from && key < to);
-            }
+            for (int d = 0; d < SUB; ++d)
+                shared_tma_load_if(dst + d * (kSlice * 128), (j & 1) ? &tm_v : &tm_k, 64 * d, hk, at, bar, leader);
         }
-        cp_commit();
         f_slot = f_slot + 1 == ST ? 0 : f_slot + 1;
     };
 #pragma unroll
     for (int j = 0; j < ST - 1; ++j) fetch(j);
-    const float scale2 = p.scale * kSharedLog2e;
-    int slot = 0;
+    const bool plain = p.softcap <= 0.f && p.scale > 0.f;  // the maximum is taken over the raw products
+    const float s2 = plain ? p.scale * kSharedLog2e : 1.f;
+    // ldmatrix offsets of this lane in a [16 keys][128 bytes] box, for the four 32-byte columns
+    uint32_t k_off[4], v_off[4];
+    {
+        const int kk = (lane & 7) + ((lane >> 4) << 3), kh = (lane >> 3) & 1, vk = lane & 15, vh = lane >> 4;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            k_off[c] = kk * 128 + (((2 * c + kh) ^ (kk & 7)) << 4);
+            v_off[c] = vk * 128 + (((2 * c + vh) ^ (vk & 7)) << 4);
+        }
+    }
+    int slot = 0, phase = 0;
     for (int i = 0; i < mine; ++i) {
         fetch(2 * i + ST - 1);
-        cp_wait<ST - 1>();
-        __syncwarp();
-        const uint32_t kt = ring + slot * SP::kHalf;
-        slot = slot + 1 == ST ? 0 : slot + 1;
         const int s = s0 + warp + i * kWarps;
         const bool in_a = s < ka.slices;
         const int key0 = in_a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
         const int lo = in_a ? ka.lo : kb.lo, hi = in_a ? ka.hi : kb.hi, base = in_a ? 0 : p.prefix_len;
         // scores of 16 rows x 16 keys: this lane's rows g, g + 8 and keys c2, c2 + 1 (+ 8)
-        float s0v[4] = {0.f, 0.f, 0.f, 0.f}, s1v[4] = {0.f, 0.f, 0.f, 0.f};
+        float v[8];
         {
-            const int key = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+            shared_warp_wait(ok, full + 8 * slot, phase, &g_shared_small_wait_timeouts);
+            const uint32_t kt = ring + slot * SP::kHalf;
+            float s0v[4] = {0.f, 0.f, 0.f, 0.f}, s1v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t b0, b1, b2, b3;
-                ldsm_x4(kt + key * (HD * 2) + (((2 * k + half) ^ (key & 7)) << 4), b0, b1, b2, b3);
+                ldsm_x4(kt + (k >> 2) * (kSlice * 128) + k_off[k & 3], b0, b1, b2, b3);
                 mma_bf16_16816(s0v, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b0, b1);
                 mma_bf16_16816(s1v, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b2, b3);
             }
+            v[0] = s0v[0], v[1] = s0v[1], v[2] = s1v[0], v[3] = s1v[1];
+            v[4] = s0v[2], v[5] = s0v[3], v[6] = s1v[2], v[7] = s1v[3];
+            if (++slot == ST) slot = 0, phase ^= 1;
         }
-        auto shape = [&](float dot, int key, int pos) {
-            const float sc = p.softcap > 0.f ? p.softcap * kSharedLog2e * tanhf(dot * p.scale / p.softcap) : dot * scale2;
-            const int kp = base + key;
-            const bool see = key >= lo && key < hi && kp <= pos && (p.window == 0 || kp > pos - p.window);
-            return see ? sc : -INFINITY;
-        };
-        float v[8];
+        if (!plain) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            v[j] = shape(s0v[j], key0 + c2 + j, posA);
-            v[2 + j] = shape(s1v[j], key0 + 8 + c2 + j, posA);
-            v[4 + j] = shape(s0v[2 + j], key0 + c2 + j, posB);
-            v[6 + j] = shape(s1v[2 + j], key0 + 8 + c2 + j, posB);
+            for (int j = 0; j < 8; ++j)
+                v[j] = kSharedLog2e * (p.softcap > 0.f ? p.softcap * tanhf(v[j] * p.scale / p.softcap) : v[j] * p.scale);
+        }
+        const bool inside = key0 >= lo && key0 + kSlice <= hi;
+        if (!(inside && base + key0 + kSlice - 1 <= pmin && (p.window == 0 || base + key0 > pmax - p.window))) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = key0 + c2 + (j & 1) + ((j & 2) << 2), kp = base + key, pos = j < 4 ? posA : posB;
+                if (!(key >= lo && key < hi && kp <= pos && (p.window == 0 || kp > pos - p.window))) v[j] = -INFINITY;
+            }
         }
         float xA = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), xB = fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]));
 #pragma unroll
@@ -319,11 +318,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) shared_attn_small_kernel(const
             xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, w));
             xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, w));
         }
-        const float nA = fmaxf(mA, xA), nB = fmaxf(mB, xB);
-        // a row that has seen no key keeps m = -inf; 0 stands in so that no inf - inf appears
-        const float zA = nA == -INFINITY ? 0.f : nA, zB = nB == -INFINITY ? 0.f : nB;
-        if (__any_sync(0xffffffffu, nA != mA || nB != mB)) {
-            const float aA = shared_ex2(mA - zA), aB = shared_ex2(mB - zB);
+        xA *= s2;
+        xB *= s2;
+        // the reference of a row: its first maximum, moved when outgrown by 2^40 (fp32's exponent
+        // range carries the rest). A row that has seen no key keeps -inf; 0 stands in below, so that
+        // no inf - inf appears.
+        const bool upA = xA > mA + kSharedLazy || (mA == -INFINITY && xA > -INFINITY);
+        const bool upB = xB > mB + kSharedLazy || (mB == -INFINITY && xB > -INFINITY);
+        if (__any_sync(0xffffffffu, upA || upB)) {
+            const float nA = upA ? xA : mA, nB = upB ? xB : mB;
+            const float aA = upA ? shared_ex2(mA - nA) : 1.f, aB = upB ? shared_ex2(mB - nB) : 1.f;
             lA *= aA;
             lB *= aB;
 #pragma unroll
@@ -336,34 +340,49 @@ __global__ void __launch_bounds__(kWarps * 32, 2) shared_attn_small_kernel(const
             mA = nA;
             mB = nB;
         }
+        const float zA = mA == -INFINITY ? 0.f : mA, zB = mB == -INFINITY ? 0.f : mB;
         uint32_t pf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float z = j < 2 ? zA : zB;
-            pf[j] = pack_bf2(f2bf(shared_ex2(v[2 * j] - z)), f2bf(shared_ex2(v[2 * j + 1] - z)));
+            pf[j] = shared_pack(shared_ex2(fmaf(v[2 * j], s2, -z)), shared_ex2(fmaf(v[2 * j + 1], s2, -z)));
             const float sum = __uint_as_float(pf[j] << 16) + __uint_as_float(pf[j] & 0xffff0000u);
             if (j < 2) lA += sum;
             else lB += sum;
         }
-        __syncwarp();  // every lane has read the K stage that the next fetch refills
+        __syncwarp();  // every lane has read the K stage that the next copy refills
         fetch(2 * i + ST);
-        cp_wait<ST - 1>();
-        __syncwarp();
-        const uint32_t vt = ring + slot * SP::kHalf;
-        slot = slot + 1 == ST ? 0 : slot + 1;
         {
-            const int key = lane & 15, half = lane >> 4;
+            shared_warp_wait(ok, full + 8 * slot, phase, &g_shared_small_wait_timeouts);
+            const uint32_t vt = ring + slot * SP::kHalf;
+            if (!inside) {
+                const int head = min(kSlice, max(0, lo - key0)), tail = max(0, min(kSlice, hi - key0));  // rows before, from
+                const int n = tail <= head ? kSlice : head + kSlice - tail;
+                for (int j = lane; j < n * SUB * 8; j += 32) {
+                    const int r = j / (SUB * 8), key = tail <= head || r < head ? r : tail + r - head, ch = j % (SUB * 8);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (ch >> 3) * (kSlice * 128) + key * 128 + (ch & 7) * 16),
+                                 "r"(0)
+                                 : "memory");
+                }
+                fence_proxy_async();  // before a later copy into the stage
+                __syncwarp();
+            }
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) {
                 uint32_t b0, b1, b2, b3;
-                ldsm_x4_t(vt + key * (HD * 2) + (((2 * d + half) ^ (key & 7)) << 4), b0, b1, b2, b3);
+                ldsm_x4_t(vt + (d >> 2) * (kSlice * 128) + v_off[d & 3], b0, b1, b2, b3);
                 mma_bf16_16816(o[2 * d], pf[0], pf[2], pf[1], pf[3], b0, b1);
                 mma_bf16_16816(o[2 * d + 1], pf[0], pf[2], pf[1], pf[3], b2, b3);
             }
+            if (++slot == ST) slot = 0, phase ^= 1;
         }
         __syncwarp();  // and the V stage
     }
-    cp_wait<0>();
+    if (!ok) {
+        // a wait gave up: give copies that may still be in flight the same time again
+        const uint64_t from = shared_now_ns();
+        while (shared_now_ns() - from < 500000000ull) __nanosleep(1000);
+    }
 #pragma unroll
     for (int w = 1; w <= 2; w <<= 1) {
         lA += __shfl_xor_sync(0xffffffffu, lA, w);
@@ -517,8 +536,10 @@ void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, const Shar
     if (pl.tc_splits > 0) launch_shared_attn_tc(p, pl, parts, stream);
     if (n_prefix + n_req > 0) {
         allow_smem(reinterpret_cast<const void*>(shared_attn_small_kernel<HD>), SP::kSmem);
+        CUtensorMap tk, tv;
+        shared_pool_maps(p, kSlice, &tk, &tv);
         shared_launch(shared_attn_small_kernel<HD>, static_cast<unsigned>(n_prefix + n_req), kWarps * 32, SP::kSmem, stream,
-                      pl.tc_splits > 0, p, pl, parts, pl.tc_splits > 0 ? 1 : 0);
+                      pl.tc_splits > 0, tk, tv, p, pl, parts, pl.tc_splits > 0 ? 1 : 0);
     }
     if (parts.direct) return;  // the only part wrote the output
     // one warp joins a few parts as fast as several: the loads of four are in flight at once
@@ -551,6 +572,12 @@ void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
         case 256: launch_shared_t<256>(p, pl, parts, stream); break;
         default: throw ArgError("sdpa_shared_prefix: head_dim must be 64, 128 or 256");
     }
+}
+
+int64_t read_shared_attn_wait_timeouts() {
+    int a = 0;
+    HYB_CUDA(cudaMemcpyFromSymbol(&a, g_shared_small_wait_timeouts, sizeof(int)));
+    return a + read_shared_attn_tc_wait_timeouts();
 }
 
 }  // namespace hyb

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "kernels.h"
+#include "tma.cuh"
 
 #include <utility>
 
@@ -10,6 +11,7 @@ namespace hyb {
 
 constexpr float kSharedLog2e = 1.4426950408889634f;
 constexpr int kTcRows = 128;
+constexpr float kSharedLazy = 40.f;  // log2 of how far a row's maximum may outgrow its reference
 
 __device__ __forceinline__ float shared_ex2(float x) {
     float y;
@@ -17,6 +19,55 @@ __device__ __forceinline__ float shared_ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ bool shared_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ uint64_t shared_now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ uint32_t shared_pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Waits for the phase of this parity, for half a second at most. A thread that gave up once
+// (ok is false) waits no more, so a launch whose copies never land ends after about that.
+__device__ __forceinline__ void shared_wait(bool& ok, uint32_t bar, uint32_t parity, int* timeouts) {
+    if (!ok || shared_try_wait(bar, parity)) return;
+    const uint64_t t0 = shared_now_ns();
+    do {
+        if (shared_try_wait(bar, parity)) return;
+    } while (shared_now_ns() - t0 < 500000000ull);
+    atomicAdd(timeouts, 1);
+    ok = false;
+}
+
+// The same by a whole warp, which goes on as one.
+__device__ __forceinline__ void shared_warp_wait(bool& ok, uint32_t bar, uint32_t parity, int* timeouts) {
+    if (!ok || __all_sync(0xffffffffu, shared_try_wait(bar, parity))) return;
+    const uint64_t t0 = shared_now_ns();
+    do {
+        if (__all_sync(0xffffffffu, shared_try_wait(bar, parity))) return;
+    } while (__all_sync(0xffffffffu, shared_now_ns() - t0 < 500000000ull));
+    if ((threadIdx.x & 31) == 0) atomicAdd(timeouts, 1);
+    ok = false;
+}
+
+// Issued by the lane whose `leader` is set, of a warp that goes on as one: a copy issued lane by
+// lane with lane-dependent coordinates takes over 100 cycles.
+__device__ __forceinline__ void shared_tma_load_if(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %6, 0;\n"
+        " @q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(leader)
+        : "memory");
+}
 // How a call's rows and keys are split; the same on the host for the scratch size and the
 // grids, and on the device. Parts of a row, in this order: those of the 128-row kernel, the
 // prefix's and the request's own ones of the 16-row kernel.
@@ -70,5 +121,9 @@ void shared_launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t s
 }
 
 void launch_shared_attn_tc(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream);
+int64_t read_shared_attn_tc_wait_timeouts();
+
+// Tensor maps of the pools: boxes of 64 head_dim columns of one KV head x `box_slots` slots.
+void shared_pool_maps(const SharedAttnParams& p, int box_slots, CUtensorMap* tk, CUtensorMap* tv);
 
 }  // namespace hyb

@@ -42,7 +42,6 @@ constexpr int kSoftWarps = 8;
 constexpr int kGroupWarps = 4;
 constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 2;  // two producers: K, V
 constexpr int kThreads = kSoftWarps * 32 + 96;
-constexpr float kLazy = 40.f;  // log2 of how far a row's maximum may outgrow its reference
 
 // Shared memory: the ring of K and V blocks and two P blocks. The queries are in TMEM: as a
 // shared-memory operand they would be read again for every block (64 KB of 224 KB a block at
@@ -62,40 +61,11 @@ struct TcShared {
     static constexpr int kSmem = kOffBars + 384 + 1024;      // + alignment slack
 };
 
-__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(done)
-                 : "r"(bar), "r"(parity)
-                 : "memory");
-    return done != 0;
-}
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// Waits for the phase of this parity, for half a second at most. A thread that gave up once
-// (ok is false) waits no more, so a launch whose copies never land ends after about that.
 __device__ __forceinline__ void wait_b(bool& ok, uint32_t bar, uint32_t parity) {
-    if (!ok || try_wait(bar, parity)) return;
-    const uint64_t t0 = now_ns();
-    do {
-        if (try_wait(bar, parity)) return;
-    } while (now_ns() - t0 < 500000000ull);
-    atomicAdd(&g_shared_attn_wait_timeouts, 1);
-    ok = false;
+    shared_wait(ok, bar, parity, &g_shared_attn_wait_timeouts);
 }
-
-// The same by a whole warp, which goes on as one.
 __device__ __forceinline__ void warp_wait(bool& ok, uint32_t bar, uint32_t parity) {
-    if (!ok || __all_sync(0xffffffffu, try_wait(bar, parity))) return;
-    const uint64_t t0 = now_ns();
-    do {
-        if (__all_sync(0xffffffffu, try_wait(bar, parity))) return;
-    } while (__all_sync(0xffffffffu, now_ns() - t0 < 500000000ull));
-    if ((threadIdx.x & 31) == 0) atomicAdd(&g_shared_attn_wait_timeouts, 1);
-    ok = false;
+    shared_warp_wait(ok, bar, parity, &g_shared_attn_wait_timeouts);
 }
 
 // Instruction descriptor: bf16 A and B, f32 D; B MN-major when b_mn.
@@ -138,15 +108,6 @@ __device__ __forceinline__ void mma_smem_a(uint32_t d_tmem, uint32_t a_lo, uint3
         "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHi)
         : "memory");
 }
-// Issued by the lane whose `leader` is set, of a warp that goes on as one: a copy issued lane by
-// lane with lane-dependent coordinates takes over 100 cycles.
-__device__ __forceinline__ void tma_load_if(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar, uint32_t leader) {
-    asm volatile(
-        "{\n .reg .pred q;\n setp.ne.u32 q, %6, 0;\n"
-        " @q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(leader)
-        : "memory");
-}
 __device__ __forceinline__ void commit_if(uint32_t bar, uint32_t leader) {
     asm volatile(
         "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
@@ -163,10 +124,6 @@ __device__ __forceinline__ void st_v8(float* p, const uint32_t* r) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
                  "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
-}
-__device__ __forceinline__ uint32_t pack_rn(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // The keys of one segment (prefix or own) that a tile of rows sees: [lo, hi), in 64-key blocks.
@@ -357,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int row = __shfl_sync(0xffffffffu, at, (c % per_load) * pieces + q);
 #pragma unroll
                 for (int d = 0; d < SUB; ++d)
-                    tma_load_if(dst + d * (kKeys * 128) + ((q << shift) << 7), map, 64 * d, hk, row, slot_full + 8 * slot, leader);
+                    shared_tma_load_if(dst + d * (kKeys * 128) + ((q << shift) << 7), map, 64 * d, hk, row, slot_full + 8 * slot, leader);
             }
         }
     } else if (warp == kMmaWarp) {
@@ -390,14 +347,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             // read it, and the group finds it ready when it is through with block c
             for (int c = 0; c < nb; ++c) {
                 const int sb = c & 1;
-                const bool v_here = try_wait(slot_full + 8 * vs, vph);  // asked for ahead of its use
+                const bool v_here = shared_try_wait(slot_full + 8 * vs, vph);  // asked for ahead of its use
                 if (c + 2 < nb) {
                     ks += 2;
                     if (ks >= SLOTS) {
                         ks -= SLOTS;
                         kph ^= 1;
                     }
-                    const bool k_here = try_wait(slot_full + 8 * ks, kph);
+                    const bool k_here = shared_try_wait(slot_full + 8 * ks, kph);
                     warp_wait(ok, s_empty + 8 * sb, (c >> 1) & 1);
                     if (!__all_sync(0xffffffffu, k_here)) warp_wait(ok, slot_full + 8 * ks, kph);
                     issue_s(sb, ks);
@@ -477,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 take_over(other);
                 ref = s_ref[r];
             }
-            const bool move = mx > ref + kLazy || (ref == -INFINITY && mx > -INFINITY);
+            const bool move = mx > ref + kSharedLazy || (ref == -INFINITY && mx > -INFINITY);
             const float now = move ? mx : ref;
             if (c + 1 < nb) {
                 s_ref[r] = now;
@@ -512,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                w[i] = pack_rn(shared_ex2(fmaf(x[2 * i], s2, -z)), shared_ex2(fmaf(x[2 * i + 1], s2, -z)));
+                w[i] = shared_pack(shared_ex2(fmaf(x[2 * i], s2, -z)), shared_ex2(fmaf(x[2 * i + 1], s2, -z)));
                 sum[(2 * i) & 3] += __uint_as_float(w[i] << 16);
                 sum[(2 * i + 1) & 3] += __uint_as_float(w[i] & 0xffff0000u);
             }
@@ -594,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (r < rows && pos >= 0) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] = pack_rn(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    for (int i = 0; i < 16; ++i) w[i] = shared_pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
                     st_v8(reinterpret_cast<float*>(dst + col / 2), w);
                     st_v8(reinterpret_cast<float*>(dst + col / 2 + 8), w + 8);
                 }
@@ -603,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) {
         // a wait gave up: give copies and MMAs that may still be in flight the same time again
-        const uint64_t t0 = now_ns();
-        while (now_ns() - t0 < 500000000ull) __nanosleep(1000);
+        const uint64_t t0 = shared_now_ns();
+        while (shared_now_ns() - t0 < 500000000ull) __nanosleep(1000);
     }
     tc_fence_before();
     __syncthreads();
@@ -618,11 +575,7 @@ template <int HD>
 void launch_t(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream) {
     using S = TcShared<HD>;
     CUtensorMap tk, tv;
-    const uint64_t dims[3] = {HD, static_cast<uint64_t>(p.n_kv), static_cast<uint64_t>(p.n_pages) * p.page_size};
-    const uint64_t strides[2] = {HD * 2, static_cast<uint64_t>(p.n_kv) * HD * 2};
-    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(p.page_size < kKeys ? p.page_size : kKeys)};
-    encode_tma(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.k_pool, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    encode_tma(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.v_pool, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    shared_pool_maps(p, p.page_size < kKeys ? p.page_size : kKeys, &tk, &tv);
     allow_smem(reinterpret_cast<const void*>(shared_attn_tc_kernel<HD>), S::kSmem);
     const long long ctas = static_cast<long long>(pl.tc_tiles) * (pl.tc_per_request ? p.n_req : 1) * p.n_kv * pl.tc_splits;
     if (ctas > INT_MAX) throw ArgError("sdpa_shared_prefix: too many parts");
@@ -632,6 +585,14 @@ void launch_t(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts
 
 }  // namespace
 
+void shared_pool_maps(const SharedAttnParams& p, int box_slots, CUtensorMap* tk, CUtensorMap* tv) {
+    const uint64_t hd = static_cast<uint64_t>(p.hd), dims[3] = {hd, static_cast<uint64_t>(p.n_kv), static_cast<uint64_t>(p.n_pages) * p.page_size};
+    const uint64_t strides[2] = {hd * 2, static_cast<uint64_t>(p.n_kv) * hd * 2};
+    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(box_slots)};
+    encode_tma(tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.k_pool, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    encode_tma(tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.v_pool, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 void launch_shared_attn_tc(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream) {
     switch (p.hd) {
         case 64: launch_t<64>(p, pl, parts, stream); break;
@@ -640,7 +601,7 @@ void launch_shared_attn_tc(const SharedAttnParams& p, const SharedPlan& pl, cons
     }
 }
 
-int64_t read_shared_attn_wait_timeouts() {
+int64_t read_shared_attn_tc_wait_timeouts() {
     int a = 0;
     HYB_CUDA(cudaMemcpyFromSymbol(&a, g_shared_attn_wait_timeouts, sizeof(int)));
     return a;

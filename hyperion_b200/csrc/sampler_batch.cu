@@ -14,19 +14,27 @@
 // d = n/32 + r with |r| <= 1/64, 2^r by its Taylor polynomial of degree 5 in r ln 2 (the next
 // term is below (ln 2 / 64)^6 / 720 = 2e-15), 2^(j/32) from a 32-entry table.
 //
-// One thread-block cluster per row; CTA c of the cluster owns a contiguous slice of the row,
-// loaded once into its shared memory, so the row's bytes cross HBM once and every later pass
-// runs from shared memory. The cut of top-k / top-p is found by radix selection on an
-// order-preserving 32-bit key, 11 bits a level: each CTA fills a histogram of counts and
-// weights (three 16-bit limbs, so that the shared atomics stay native 32-bit ones), the
-// cluster's first CTA adds the histograms up over distributed shared memory and finds the bin
-// in which the cut lies. bf16 logits have 16-bit keys and need two levels, fp32 ones three.
+// One thread-block cluster per row; CTA c of the cluster owns a contiguous slice of the row.
+//
+// bf16 logits (sample_hist_kernel): a bf16 value is one of 65536, so one pass over the row
+// counts every value in shared memory (16-bit counters, 128 KB, indexed by the raw bits: one
+// native shared atomic an element) and everything but the position of the token follows
+// exactly from the counts: the weight of the row, the cut of the three filters, the kept
+// weight and the draw's target. A second pass over the row (from L2) then looks for the
+// target in index order; it compares eight logits at a time with the cut and evaluates weights
+// only for kept ones. HBM sees the row once.
+//
+// fp32 logits (sample_radix_kernel): the slice is held in shared memory, and the cut of
+// top-k / top-p is found by radix selection on an order-preserving 32-bit key, 11 bits a level:
+// each CTA fills a histogram of counts and weights (three 16-bit limbs, so that the shared
+// atomics stay native 32-bit ones), the cluster's first CTA adds the histograms up over
+// distributed shared memory and finds the bin in which the cut lies.
 #include "kernels.h"
 #include "tma.cuh"
 
 #include <algorithm>
 #include <cstddef>
-#include <type_traits>
+#include <utility>
 
 namespace hyb {
 
@@ -38,7 +46,7 @@ constexpr int kBins = 2048;
 constexpr int kFrac = 44;
 constexpr int kMaxCluster = 8;
 constexpr int kSliceBytes = 128 * 1024;  // the largest slice held in shared memory
-constexpr int kMaxSlice = 65536;         // limb sums of a slice fit 32 bits: 65535 * 65536 < 2^32
+// A slice has at most 2^19 / 8 = 65536 logits, so its limb sums fit 32 bits: 65535 * 65536 < 2^32.
 
 typedef unsigned long long u64;
 
@@ -101,19 +109,13 @@ __device__ __forceinline__ uint4 cl_ld128(uint32_t a) {
 
 // NaN -> -inf, -0 -> +0.
 __device__ __forceinline__ float canon(float x) { return x != x ? -INFINITY : x + 0.0f; }
-__device__ __forceinline__ float load_x(const bf16* x, int i) { return canon(bf2f(x[i])); }
-__device__ __forceinline__ float load_x(const float* x, int i) { return canon(x[i]); }
-// Order-preserving key; a bf16 value's lies in the upper 16 bits, the rest zero.
-template <bool F32>
+// Order-preserving key.
 __device__ __forceinline__ uint32_t key_of(float f) {
     const uint32_t u = __float_as_uint(f);
-    const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return F32 ? k : k & 0xffff0000u;
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float value_of(uint32_t key, bool f32) {
-    if (key & 0x80000000u) return __uint_as_float(key & 0x7fffffffu);
-    const uint32_t u = ~key;
-    return __uint_as_float(f32 ? u : u & 0xffff0000u);
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
 // rint(2^44 * exp((x - M) / T)), c = log2(e) / T.
@@ -159,19 +161,17 @@ __device__ __forceinline__ V block_incl(V v, V* red, V* total) {
     return before + v;
 }
 
-template <bool F32>
-__global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatchParams p, int slice, int resident) {
-    using T = typename std::conditional<F32, float, bf16>::type;
+__global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatchParams p, int slice, int resident) {
     extern __shared__ __align__(16) unsigned char dyn[];
     __shared__ Share sh;
     Hist& h = *reinterpret_cast<Hist*>(dyn);
-    T* buf = reinterpret_cast<T*>(dyn + sizeof(Hist));
+    float* buf = reinterpret_cast<float*>(dyn + sizeof(Hist));
     uint32_t nc;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nc));
     const uint32_t rank = cl_rank();
     const int row = blockIdx.x / nc, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int lo = min(p.vocab, static_cast<int>(rank) * slice), n = min(p.vocab, lo + slice) - lo;
-    const T* gx = static_cast<const T*>(p.logits) + row * p.ld + lo;
+    const float* gx = static_cast<const float*>(p.logits) + row * p.ld + lo;
 
     const float temp = p.temperature ? p.temperature[row] : 1.f;
     const bool greedy = !(temp > 0.f);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
     {
         float bx = -INFINITY;
         int bi = -1;
-        constexpr int VEC = 16 / sizeof(T);
+        constexpr int VEC = 4;
         const bool vec = (reinterpret_cast<uintptr_t>(gx) & 15) == 0;
         const int nv = vec ? n / VEC : 0;
         for (int i = tid; i < nv; i += kThreads) {
@@ -195,9 +195,7 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                float x;
-                if constexpr (F32) x = canon(__uint_as_float(w[j]));
-                else x = canon(__uint_as_float((j & 1) ? w[j / 2] & 0xffff0000u : w[j / 2] << 16));
+                const float x = canon(__uint_as_float(w[j]));
                 if (bi < 0 || x > bx) {
                     bx = x;
                     bi = i * VEC + j;
@@ -205,15 +203,14 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
             }
         }
         for (int i = nv * VEC + tid; i < n; i += kThreads) {
-            const T v = gx[i];
-            if (resident) buf[i] = v;
-            const float x = load_x(&v, 0);
+            const float x = canon(gx[i]);
+            if (resident) buf[i] = x;
             if (bi < 0 || x > bx) {
                 bx = x;
                 bi = i;
             }
         }
-        if (bi >= 0) best = (static_cast<u64>(key_of<F32>(bx)) << 32) | static_cast<uint32_t>(~(lo + bi));
+        if (bi >= 0) best = (static_cast<u64>(key_of(bx)) << 32) | static_cast<uint32_t>(~(lo + bi));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -227,8 +224,8 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
     cl_sync();
     for (uint32_t r = 0; r < nc; ++r) best = max(best, cl_ld64(cl_map(&sh.best, r)));
     const uint32_t arg = ~static_cast<uint32_t>(best);
-    const float M = value_of(static_cast<uint32_t>(best >> 32), F32);
-    const T* x = resident ? buf : gx;
+    const float M = value_of(static_cast<uint32_t>(best >> 32));
+    const float* x = resident ? buf : gx;
     const bool empty = M == -INFINITY;
     if (greedy || empty) {
         if (rank == 0 && tid == 0) {
@@ -247,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
         uint32_t above = 0;
         u64 mass_above = 0, target = 0;
         uint32_t in_bin = 0;
-        constexpr int LEVELS = F32 ? 3 : 2;
+        constexpr int LEVELS = 3;
 #pragma unroll 1
         for (int level = 0; level < LEVELS; ++level) {
             const int shift = level == 0 ? 21 : (level == 1 ? 10 : 0);
@@ -255,8 +252,8 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
             for (int i = tid; i < 4 * kBins; i += kThreads) (&h.cnt[0])[i] = 0;
             __syncthreads();
             for (int i = tid; i < n; i += kThreads) {
-                const float xi = load_x(x, i);
-                const uint32_t key = key_of<F32>(xi);
+                const float xi = canon(x[i]);
+                const uint32_t key = key_of(xi);
                 if (level && (key >> (shift + width)) != (cut_key >> (shift + width))) continue;
                 const uint32_t bin = (key >> shift) & ((1u << width) - 1);
                 atomicAdd(&h.cnt[bin], 1u);
@@ -318,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
         uint32_t take = in_bin;
         if (use_k) take = min(take, static_cast<uint32_t>(k) - above);
         if (use_p) {
-            const u64 w = weight(value_of(cut_key, F32), M, c, sh.table);
+            const u64 w = weight(value_of(cut_key), M, c, sh.table);
             if (w) take = static_cast<uint32_t>(min(static_cast<u64>(take), (target - mass_above + w - 1) / w));
         }
         ties_kept = take;
@@ -333,8 +330,8 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
         u64 sum = 0;
         uint32_t cnt = 0, ties = 0;
         for (int i = from + lane; i < to; i += 32) {
-            const float xi = load_x(x, i);
-            const uint32_t key = key_of<F32>(xi);
+            const float xi = canon(x[i]);
+            const uint32_t key = key_of(xi);
             if (cut && key <= cut_key) {
                 ties += key == cut_key;
                 continue;
@@ -371,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
         }
     }
     cl_sync();
-    u64 tie_w = cut ? weight(value_of(cut_key, F32), M, c, sh.table) : 0;
+    u64 tie_w = cut ? weight(value_of(cut_key), M, c, sh.table) : 0;
     if (cut && !passes(tie_w)) {
         tie_w = 0;
         ties_kept = 0;
@@ -416,8 +413,8 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
     u64 sum = 0;
     uint32_t ties = 0;
     auto kept_weight = [&](int i, bool& tie) -> u64 {
-        const float xi = load_x(x, i);
-        const uint32_t key = key_of<F32>(xi);
+        const float xi = canon(x[i]);
+        const uint32_t key = key_of(xi);
         tie = cut && key == cut_key;
         if (cut && key <= cut_key) return 0;
         const u64 w = weight(xi, M, c, sh.table);
@@ -450,22 +447,434 @@ __global__ void __launch_bounds__(kThreads) sample_batch_kernel(const SampleBatc
     }
 }
 
-template <bool F32>
-void launch_t(const SampleBatchParams& p, cudaStream_t stream) {
-    const size_t elem = F32 ? 4 : 2;
-    const int most = std::min<int>(kMaxSlice, kSliceBytes / static_cast<int>(elem));
-    int nc = 1;
-    while (nc < kMaxCluster && (p.vocab + nc - 1) / nc > most) nc *= 2;
-    // more CTAs a row while the rows alone leave SMs idle and a slice is worth one
-    while (nc < kMaxCluster && p.rows * nc * 2 <= num_sms() && p.vocab / nc >= 4096) nc *= 2;
-    const int slice = ((p.vocab + nc - 1) / nc + 7) & ~7;
-    const int resident = slice <= most ? 1 : 0;
-    const size_t smem = sizeof(Hist) + (resident ? slice * elem : 0);
-    auto kern = sample_batch_kernel<F32>;
-    allow_smem(reinterpret_cast<const void*>(kern), sizeof(Hist) + kSliceBytes + 16);
+// ------------------------------------------------------------------------------ bf16
+constexpr int kHThreads = 1024;
+constexpr int kHWarps = kHThreads / 32;
+constexpr int kGroups = 2048;          // ordered groups of 32 neighbouring values
+constexpr int kHistBytes = 65536 * 2;
+constexpr int kHSlice = 65536;         // the slice's first logit is counted apart, so a counter stays below 2^16
+
+// Values in descending order: place o in [0, 65536) <-> raw bits. Positive ones (NaNs above +inf
+// first, whose counts are moved to -inf), then negative ones; -0 (0x8000) has the place after +0.
+__device__ __forceinline__ uint32_t raw_of(uint32_t o) { return o < 32768u ? 32767u - o : o; }
+__device__ __forceinline__ uint32_t place_of(uint32_t raw) { return raw < 32768u ? 32767u - raw : raw; }
+constexpr uint32_t kPlaceNegInf = 0xff80u, kPlaceZero = 32767u, kPlaceNegZero = 0x8000u;
+__device__ __forceinline__ bool is_nan_place(uint32_t o) { return (raw_of(o) & 0x7fffu) > 0x7f80u; }
+__device__ __forceinline__ float value_at(uint32_t o) { return __uint_as_float(raw_of(o) << 16); }
+
+struct HShare {
+    double table[32];
+    u64 mass[kGroups];       // (first CTA) weight of a group
+    uint32_t cnt[kGroups];   // (first CTA) its count
+    u64 red[kHWarps];
+    uint32_t red32[kHWarps];
+    float maxv;              // of this CTA's slice
+    uint32_t first_raw;      // its first logit
+    uint32_t cut, ties;      // (first CTA) the last kept value's place, how many of it are kept
+    uint32_t kept;
+    u64 total;               // kept weight
+    u64 sum;                 // of this CTA: kept weight above the cut
+    uint32_t tied;           // logits at the cut
+    u64 wsum[kHWarps];
+    uint32_t wties[kHWarps];
+};
+
+template <typename V>
+__device__ __forceinline__ V h_scan(V v, V* red, V* total) {  // inclusive, in thread order
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = v;
+    __syncthreads();
+    V before = lane < kHWarps ? red[lane] : V(0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V n = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += n;
+    }
+    *total = __shfl_sync(0xffffffffu, before, 31);
+    before = __shfl_sync(0xffffffffu, before, (warp + 31) & 31);
+    return (warp ? before : V(0)) + v;
+}
+
+__global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleBatchParams p, int slice) {
+    extern __shared__ __align__(16) unsigned char dyn[];
+    uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);
+    HShare& sh = *reinterpret_cast<HShare*>(dyn + kHistBytes);
+    uint32_t nc;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nc));
+    const uint32_t rank = cl_rank();
+    const int row = blockIdx.x / nc, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lo = min(p.vocab, static_cast<int>(rank) * slice), n = min(p.vocab, lo + slice) - lo;
+    const bf16* gx = static_cast<const bf16*>(p.logits) + row * p.ld + lo;
+    const uint16_t* raw16 = reinterpret_cast<const uint16_t*>(gx);
+    // 16-byte vectors from the first aligned logit on; `head` logits stand before it
+    const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(gx) & 15)) & 15) / 2);
+    const int nv = (n - head) / 8, tail = head + 8 * nv;
+    const uint4* vec = reinterpret_cast<const uint4*>(gx + head);
+
+    const float temp = p.temperature ? p.temperature[row] : 1.f;
+    const bool greedy = !(temp > 0.f);
+    const int k = p.top_k ? p.top_k[row] : 0;
+    const float tp = p.top_p ? p.top_p[row] : 0.f, mp = p.min_p ? p.min_p[row] : 0.f, u = p.u[row];
+    const bool use_k = k > 0 && k < p.vocab, use_p = tp > 0.f && tp < 1.f, use_m = mp > 0.f;
+    const double c = 1.4426950408889634074 / static_cast<double>(temp);
+
+    for (int i = tid; i < kHistBytes / 16; i += kHThreads) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+    if (tid < 32) sh.table[tid] = exp2(tid * (1.0 / 32.0));
+    __syncthreads();
+
+    // ---- count the slice's values; its maximum
+    {
+        auto count = [&](uint32_t raw) { atomicAdd(&hist[raw >> 1], (raw & 1u) ? 65536u : 1u); };
+        __nv_bfloat162 mx = __halves2bfloat162(__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80));
+        auto word = [&](uint32_t w) { mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w)); };  // a NaN loses
+        const bool all = !greedy;  // the first maximum needs no counts
+        constexpr int U = 4;
+        for (int i0 = tid; i0 < nv; i0 += U * kHThreads) {
+            uint4 v[U];
+#pragma unroll
+            for (int q = 0; q < U; ++q)
+                if (i0 + q * kHThreads < nv) v[q] = vec[i0 + q * kHThreads];
+#pragma unroll
+            for (int q = 0; q < U; ++q) {
+                const int i = i0 + q * kHThreads;
+                if (i >= nv) break;
+                const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    word(w[j]);
+                    if (all) {
+                        if (head + 8 * i + 2 * j > 0) count(w[j] & 0xffffu);
+                        count(w[j] >> 16);
+                    }
+                }
+            }
+        }
+        for (int i = tid; i < n - 8 * nv; i += kHThreads) {  // what the vectors leave at both ends
+            const int at = i < head ? i : tail + i - head;
+            const uint32_t raw = raw16[at];
+            word(raw | raw << 16);
+            if (all && at > 0) count(raw);
+        }
+        float m = fmaxf(__low2float(mx), __high2float(mx));
+        m = warp_max(m);
+        if (lane == 0) sh.red32[warp] = __float_as_uint(m);
+        __syncthreads();
+        if (warp == 0) {
+            m = warp_max(__uint_as_float(sh.red32[lane]));
+            if (lane == 0) {
+                sh.maxv = m;
+                sh.first_raw = n > 0 ? raw16[0] : 0x10000u;
+            }
+        }
+    }
+    cl_sync();
+    float M = -INFINITY;
+    for (uint32_t r = 0; r < nc; ++r) M = fmaxf(M, __uint_as_float(cl_ld32(cl_map(&sh.maxv, r))));
+    M += 0.f;  // -0 counts as +0
+    if (M == -INFINITY) {
+        if (rank == 0 && tid == 0) {
+            p.token[row] = -1;
+            if (p.kept) p.kept[row] = 0;
+            if (p.prob) p.prob[row] = 0.f;
+        }
+        cl_sync();  // no CTA leaves while another may read its shared memory
+        return;
+    }
+    uint32_t cut = place_of(__float_as_uint(M) >> 16), ties_kept = 1, kept = 1;
+    u64 total = 1ull << kFrac;
+    if (!greedy) {
+        // ---- weight and count of every ordered group; the cluster's CTAs take them in turn. A count is
+        // that of all slices and their first logits.
+        uint32_t firsts[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) firsts[r] = r < static_cast<int>(nc) ? cl_ld32(cl_map(&sh.first_raw, r)) : 0x10000u;
+        uint32_t remote[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) remote[r] = cl_map(hist, r < static_cast<int>(nc) ? r : 0);
+        // the count of place o; NaN and -inf have no weight and count as 0 here, -0 is part of +0
+        auto count_at = [&](uint32_t raw) {
+            uint32_t s = 0;
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r)
+                if (r < static_cast<int>(nc)) {
+                    const uint32_t w = cl_ld32(remote[r] + ((raw >> 1) << 2));
+                    s += (raw & 1u ? w >> 16 : w & 0xffffu) + (firsts[r] == raw ? 1u : 0u);
+                }
+            return s;
+        };
+        auto place_count = [&](uint32_t o) -> uint32_t {
+            if (is_nan_place(o) || o == kPlaceNegZero || o == kPlaceNegInf) return 0;
+            return count_at(raw_of(o)) + (o == kPlaceZero ? count_at(0x8000u) : 0u);
+        };
+        const uint32_t mass_at = cl_map(sh.mass, 0), cnt_at = cl_map(sh.cnt, 0);
+        for (int g = rank + nc * warp; g < kGroups; g += nc * kHWarps) {
+            const uint32_t o = 32 * g + lane;
+            uint32_t cn = place_count(o);
+            u64 ms = 0;
+            if (__any_sync(0xffffffffu, cn != 0)) {
+                if (cn) ms = cn * weight(value_at(o), M, c, sh.table);
+#pragma unroll
+                for (int q = 16; q; q >>= 1) {
+                    cn += __shfl_xor_sync(0xffffffffu, cn, q);
+                    ms += __shfl_xor_sync(0xffffffffu, ms, q);
+                }
+            }
+            if (lane == 0) {
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mass_at + 8 * g), "l"(ms) : "memory");
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cnt_at + 4 * g), "r"(cn) : "memory");
+            }
+        }
+        cl_sync();
+        if (rank == 0) {
+            // two groups a thread, in order; then the group that holds the cut, a value a lane
+            const uint32_t c0 = sh.cnt[2 * tid], c1 = sh.cnt[2 * tid + 1];
+            const u64 m0 = sh.mass[2 * tid], m1 = sh.mass[2 * tid + 1];
+            uint32_t cfin;
+            u64 z;
+            uint32_t cb = h_scan<uint32_t>(c0 + c1, sh.red32, &cfin) - c0 - c1;
+            u64 mb = h_scan<u64>(m0 + m1, sh.red, &z) - m0 - m1;
+            // the kept prefix ends at: the k-th token; the first at which the weight reaches top_p of
+            // all (an integer >= top_p * Z); the last with a weight of min_p
+            const u64 target = use_p ? max(1ull, static_cast<u64>(ceil(static_cast<double>(tp) * static_cast<double>(z)))) : ~0ull;
+            const u64 most = use_k ? static_cast<u64>(k) : ~0ull;
+            auto reached = [&](uint32_t cc, u64 mm) { return cc >= most || mm >= target; };
+            const bool any_cut = reached(cfin, z);
+            if (tid == 0) {
+                sh.cut = 65536u;  // nothing is cut: all tokens are kept, the -inf ones (weight 0) included
+                sh.ties = 0;
+                sh.kept = static_cast<uint32_t>(p.vocab);
+                sh.total = z;
+                if (use_k && !any_cut) sh.kept = static_cast<uint32_t>(k);  // the cut lies among the -inf ones
+            }
+            __syncthreads();
+            if (any_cut && !reached(cb, mb) && reached(cb + c0 + c1, mb + m0 + m1)) {
+                const bool second = !reached(cb + c0, mb + m0);
+                sh.red32[0] = 2 * tid + second;
+                sh.red32[1] = second ? cb + c0 : cb;
+                sh.red[0] = second ? mb + m0 : mb;
+            }
+            __syncthreads();
+            if (any_cut && warp == 0) {
+                const uint32_t o = 32 * sh.red32[0] + lane;
+                const uint32_t cn = place_count(o);
+                const u64 w = cn ? weight(value_at(o), M, c, sh.table) : 0, ms = cn * w;
+                uint32_t ci = cn;
+                u64 mi = ms;
+#pragma unroll
+                for (int q = 1; q < 32; q <<= 1) {
+                    const uint32_t a = __shfl_up_sync(0xffffffffu, ci, q);
+                    const u64 b = __shfl_up_sync(0xffffffffu, mi, q);
+                    if (lane >= q) {
+                        ci += a;
+                        mi += b;
+                    }
+                }
+                ci += sh.red32[1];
+                mi += sh.red[0];
+                if (!reached(ci - cn, mi - ms) && reached(ci, mi)) {
+                    u64 take = cn;
+                    if (use_k) take = min(take, most - (ci - cn));
+                    if (use_p && w) take = min(take, (target - (mi - ms) + w - 1) / w);
+                    sh.cut = o;
+                    sh.ties = static_cast<uint32_t>(take);
+                    sh.kept = ci - cn + static_cast<uint32_t>(take);
+                    sh.total = mi - ms + take * w;
+                }
+            }
+            __syncthreads();
+            if (use_m) {
+                // min-p: the kept tokens with w >= min_p; where the cut's own weight passes nothing changes
+                const double mpd = static_cast<double>(fminf(mp, 1.f)) * 17592186044416.0;
+                const uint32_t kc = sh.cut;
+                const bool cut_passes = kc < 65536u && static_cast<double>(weight(value_at(kc), M, c, sh.table)) >= mpd;
+                if (!cut_passes) {
+                    // weights fall along the places, so the passing places are a prefix, which ends before the
+                    // cut: a binary search by one thread over all 65536, then the sums of the groups before
+                    uint32_t a = 0, b = min(kc, 65536u);  // places < a pass, places >= b do not
+                    while (a < b) {
+                        const uint32_t mid = (a + b) >> 1;
+                        const float x = is_nan_place(mid) ? (mid < 32768u ? INFINITY : -INFINITY) : value_at(mid);
+                        const bool pass = x >= M || static_cast<double>(weight(x, M, c, sh.table)) >= mpd;
+                        if (pass) a = mid + 1;
+                        else b = mid;
+                    }
+                    const uint32_t end = a, ge = end >> 5;
+                    __syncthreads();
+                    if (2 * tid <= ge && ge <= 2 * tid + 1) {
+                        const bool second = ge == 2u * tid + 1;
+                        sh.red32[1] = second ? cb + c0 : cb;
+                        sh.red[0] = second ? mb + m0 : mb;
+                    }
+                    __syncthreads();
+                    if (warp == 0) {
+                        uint32_t cn = 0;
+                        u64 ms = 0;
+                        const uint32_t o = 32 * ge + lane;
+                        if (o < end) {
+                            cn = place_count(o);
+                            ms = cn ? cn * weight(value_at(o), M, c, sh.table) : 0;
+                        }
+#pragma unroll
+                        for (int q = 16; q; q >>= 1) {
+                            cn += __shfl_xor_sync(0xffffffffu, cn, q);
+                            ms += __shfl_xor_sync(0xffffffffu, ms, q);
+                        }
+                        if (lane == 0) {
+                            sh.cut = end;  // places before it are kept, none of it
+                            sh.ties = 0;
+                            sh.kept = sh.red32[1] + cn;
+                            sh.total = sh.red[0] + ms;
+                        }
+                    }
+                }
+            }
+        }
+        cl_sync();
+        cut = cl_ld32(cl_map(&sh.cut, 0));
+        ties_kept = cl_ld32(cl_map(&sh.ties, 0));
+        kept = cl_ld32(cl_map(&sh.kept, 0));
+        total = cl_ld64(cl_map(&sh.total, 0));
+    }
+    const double uw = static_cast<double>(u) * static_cast<double>(total);
+    const u64 want = greedy || !(uw >= 0.0) ? 0 : min(total - 1, static_cast<u64>(uw));  // running sum > want
+
+    // ---- second pass: kept weight of every warp's run of the slice, in index order
+    const float cut_v = cut < 65536u ? (is_nan_place(cut) ? (cut < 32768u ? INFINITY : -INFINITY) : value_at(cut) + 0.f) : -INFINITY;
+    const u64 tie_w = ties_kept ? weight(cut_v, M, c, sh.table) : 0;
+    // above: places before the cut. Without a cut everything above -inf is (weight 0 below).
+    auto look = [&](float x, bool& tie) -> u64 {
+        tie = ties_kept && x == cut_v;
+        return x > cut_v ? weight(x, M, c, sh.table) : 0;
+    };
+    const int run = ((slice + kHWarps - 1) / kHWarps + 255) & ~255;  // whole warp-wide vectors
+    {
+        const int from = warp * run, to = min(n, from + run);  // vectors and ends, counted from `head` on
+        u64 sum = 0;
+        uint32_t ties = 0;
+        const __nv_bfloat162 cut2 = __float2bfloat162_rn(cut_v);
+        // positions from..to - 1 of the slice: logit at position i
+        auto one = [&](int i) {
+            bool tie;
+            const float x = canon(bf2f(raw16[i]));
+            sum += look(x, tie);
+            ties += tie;
+        };
+        // vectors that lie wholly inside [from, to)
+        const int v0 = max(0, (from - head + 7) / 8), v1 = max(v0, (to - head) >= 0 ? (to - head) / 8 : 0);
+        if (from < to) {
+            const int a_end = min(to, head + 8 * v0), b_start = max(a_end, head + 8 * v1);
+            for (int i = from + lane; i < a_end; i += 32) one(i);
+            for (int i = b_start + lane; i < to; i += 32) one(i);
+            for (int i0 = v0 + lane; i0 < v1; i0 += 4 * 32) {
+                uint4 v[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (i0 + 32 * q < v1) v[q] = vec[i0 + 32 * q];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (i0 + 32 * q >= v1) break;
+                    const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+                    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+                    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+                    if (!__hbge2(cut2, m) || ties_kept) {
+                        // some logit lies above the cut (or may lie at it)
+                        const float ma = fmaxf(__low2float(m), __high2float(m));
+                        if (ma >= cut_v)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                bool tie;
+                                sum += look(canon(__uint_as_float(w[j] << 16)), tie);
+                                ties += tie;
+                                sum += look(canon(__uint_as_float(w[j] & 0xffff0000u)), tie);
+                                ties += tie;
+                            }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        ties = __reduce_add_sync(0xffffffffu, ties);
+        if (lane == 0) {
+            sh.wsum[warp] = sum;
+            sh.wties[warp] = ties;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            u64 s = sh.wsum[lane];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            const uint32_t t = __reduce_add_sync(0xffffffffu, sh.wties[lane]);
+            if (lane == 0) {
+                sh.sum = s;
+                sh.tied = t;
+            }
+        }
+    }
+    cl_sync();
+    u64 at = 0;          // kept weight in front of this CTA
+    uint32_t tb = 0;     // logits at the cut in front of it
+    for (uint32_t r = 0; r < rank; ++r) {
+        const u64 s = cl_ld64(cl_map(&sh.sum, r));
+        const uint32_t t = cl_ld32(cl_map(&sh.tied, r));
+        at += s + tie_w * (min(ties_kept, tb + t) - min(ties_kept, tb));
+        tb += t;
+    }
+    cl_sync();  // the cluster is done with this CTA's shared memory
+    // ---- the warp's run that holds the target, then the token in it
+    int w0 = -1;
+    for (int w = 0; w < kHWarps; ++w) {
+        const u64 s = sh.wsum[w] + tie_w * (min(ties_kept, tb + sh.wties[w]) - min(ties_kept, tb));
+        if (want >= at && want < at + s) {
+            w0 = w;
+            break;
+        }
+        at += s;
+        tb += sh.wties[w];
+    }
+    if (w0 < 0) return;  // another CTA's
+    const int from = w0 * run, to = min(n, from + run), per = (run + kHThreads - 1) / kHThreads;
+    const int i0 = min(to, from + tid * per), i1 = min(to, i0 + per);
+    u64 sum = 0;
+    uint32_t ties = 0;
+    for (int i = i0; i < i1; ++i) {
+        bool tie;
+        sum += look(canon(bf2f(raw16[i])), tie);
+        ties += tie;
+    }
+    uint32_t all_ties;
+    u64 all;
+    const uint32_t tie_at = tb + h_scan<uint32_t>(ties, sh.red32, &all_ties) - ties;
+    sum += tie_w * (min(ties_kept, tie_at + ties) - min(ties_kept, tie_at));
+    u64 acc = at + h_scan<u64>(sum, sh.red, &all) - sum;
+    if (want >= acc && want < acc + sum) {
+        uint32_t tr = tie_at;
+        for (int i = i0; i < i1; ++i) {
+            bool tie;
+            u64 w = look(canon(bf2f(raw16[i])), tie);
+            if (tie) w = tr++ < ties_kept ? tie_w : 0;
+            if (want < acc + w) {
+                p.token[row] = lo + i;
+                if (p.kept) p.kept[row] = static_cast<int>(kept);
+                if (p.prob) p.prob[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(total));
+                break;
+            }
+            acc += w;
+        }
+    }
+}
+
+template <typename... P, typename... A>
+void launch_cluster(void (*kern)(P...), int rows, int nc, int threads, size_t smem, cudaStream_t stream, A&&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * nc);
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(static_cast<unsigned>(rows) * nc);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -475,15 +884,37 @@ void launch_t(const SampleBatchParams& p, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    HYB_CUDA(cudaLaunchKernelEx(&cfg, kern, p, slice, resident));
-    HYB_LAUNCH_CHECK("sample_batch_kernel");
+    HYB_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...));
+    HYB_LAUNCH_CHECK("sample_batch kernel");
+}
+
+void launch_hist(const SampleBatchParams& p, cudaStream_t stream) {
+    // the fewest CTAs a row whose slices fit the counters; more while the rows alone leave SMs idle
+    int nc = 1;
+    while (nc < kMaxCluster && (p.vocab + nc - 1) / nc > kHSlice) nc *= 2;
+    while (nc < kMaxCluster && p.rows * nc * 2 <= num_sms() && p.vocab / nc >= 8192) nc *= 2;
+    const int slice = ((p.vocab + nc - 1) / nc + 7) & ~7;
+    allow_smem(reinterpret_cast<const void*>(sample_hist_kernel), kHistBytes + sizeof(HShare));
+    launch_cluster(sample_hist_kernel, p.rows, nc, kHThreads, kHistBytes + sizeof(HShare), stream, p, slice);
+}
+
+void launch_f32(const SampleBatchParams& p, cudaStream_t stream) {
+    const int most = kSliceBytes / 4;
+    int nc = 1;
+    while (nc < kMaxCluster && (p.vocab + nc - 1) / nc > most) nc *= 2;
+    // more CTAs a row while the rows alone leave SMs idle and a slice is worth one
+    while (nc < kMaxCluster && p.rows * nc * 2 <= num_sms() && p.vocab / nc >= 4096) nc *= 2;
+    const int slice = ((p.vocab + nc - 1) / nc + 7) & ~7;
+    const int resident = slice <= most ? 1 : 0;  // above 2^18 logits the slice stays in L2
+    allow_smem(reinterpret_cast<const void*>(sample_radix_kernel), sizeof(Hist) + kSliceBytes + 16);
+    launch_cluster(sample_radix_kernel, p.rows, nc, kThreads, sizeof(Hist) + (resident ? slice * 4 : 0), stream, p, slice, resident);
 }
 
 }  // namespace
 
 void launch_sample_batch(const SampleBatchParams& p, cudaStream_t stream) {
-    if (p.f32) launch_t<true>(p, stream);
-    else launch_t<false>(p, stream);
+    if (p.f32) launch_f32(p, stream);
+    else launch_hist(p, stream);
 }
 
 }  // namespace hyb

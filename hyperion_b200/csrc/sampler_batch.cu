@@ -18,7 +18,7 @@
 //
 // bf16 logits (sample_hist_kernel): a bf16 value is one of 65536, so one pass over the row
 // counts every value in shared memory (16-bit counters, 128 KB, indexed by the raw bits: one
-// native shared atomic an element) and everything but the position of the token follows
+// native shared atomic an element; every 2^15 logits full counters are folded into a list) and everything but the position of the token follows
 // exactly from the counts: the weight of the row, the cut of the three filters, the kept
 // weight and the draw's target. A second pass over the row (from L2) then looks for the
 // target in index order; it compares eight logits at a time with the cut and evaluates weights
@@ -452,7 +452,9 @@ constexpr int kHThreads = 1024;
 constexpr int kHWarps = kHThreads / 32;
 constexpr int kGroups = 2048;          // ordered groups of 32 neighbouring values
 constexpr int kHistBytes = 65536 * 2;
-constexpr int kHSlice = 65536;         // the slice's first logit is counted apart, so a counter stays below 2^16
+constexpr int kHSlice = 131072;
+constexpr int kFold = 32768;           // logits between two folds of the counters
+constexpr int kMaxBig = kHSlice / kFold;
 
 // Values in descending order: place o in [0, 65536) <-> raw bits. Positive ones (NaNs above +inf
 // first, whose counts are moved to -inf), then negative ones; -0 (0x8000) has the place after +0.
@@ -469,7 +471,11 @@ struct HShare {
     u64 red[kHWarps];
     uint32_t red32[kHWarps];
     float maxv;              // of this CTA's slice
-    uint32_t first_raw;      // its first logit
+    uint32_t n_big;          // counters that reached 2^15 at a fold ..
+    uint32_t big[kMaxBig];   // .. each stands for 2^15 logits of this value more
+    uint32_t map[kGroups / 32];  // groups with a count
+    uint32_t n_list;
+    uint16_t list[kGroups];      // the groups in which some CTA has a count
     uint32_t cut, ties;      // (first CTA) the last kept value's place, how many of it are kept
     uint32_t kept;
     u64 total;               // kept weight
@@ -501,14 +507,13 @@ __device__ __forceinline__ V h_scan(V v, V* red, V* total) {  // inclusive, in t
     return (warp ? before : V(0)) + v;
 }
 
+template <int NC>
 __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleBatchParams p, int slice) {
     extern __shared__ __align__(16) unsigned char dyn[];
     uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);
     HShare& sh = *reinterpret_cast<HShare*>(dyn + kHistBytes);
-    uint32_t nc;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nc));
     const uint32_t rank = cl_rank();
-    const int row = blockIdx.x / nc, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / NC, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int lo = min(p.vocab, static_cast<int>(rank) * slice), n = min(p.vocab, lo + slice) - lo;
     const bf16* gx = static_cast<const bf16*>(p.logits) + row * p.ld + lo;
     const uint16_t* raw16 = reinterpret_cast<const uint16_t*>(gx);
@@ -526,40 +531,67 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
 
     for (int i = tid; i < kHistBytes / 16; i += kHThreads) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid < 32) sh.table[tid] = exp2(tid * (1.0 / 32.0));
+    if (tid == 0) sh.n_big = 0;
     __syncthreads();
 
     // ---- count the slice's values; its maximum
     {
-        auto count = [&](uint32_t raw) { atomicAdd(&hist[raw >> 1], (raw & 1u) ? 65536u : 1u); };
+        // two values share a word: the even one's count is the lower half
+        const uint32_t hist_at = smem_u32(hist);
+        auto add = [&](uint32_t at, uint32_t inc) { asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(hist_at + at), "r"(inc) : "memory"); };
         __nv_bfloat162 mx = __halves2bfloat162(__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80));
-        auto word = [&](uint32_t w) { mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w)); };  // a NaN loses
-        const bool all = !greedy;  // the first maximum needs no counts
+        auto word = [&](uint32_t w) {
+            mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w));  // a NaN loses
+            if (!greedy) {  // the first maximum needs no counts
+                add((w << 1) & 0x1fffcu, (w & 1u) * 65535u + 1u);
+                add((w >> 15) & 0x1fffcu, ((w >> 16) & 1u) * 65535u + 1u);
+            }
+        };
         constexpr int U = 4;
-        for (int i0 = tid; i0 < nv; i0 += U * kHThreads) {
-            uint4 v[U];
+        // vectors between two folds; the up to 14 logits beside the vectors come on top of the last
+        const int chunk = n > 65535 ? kFold / 8 - 2 : nv;
+        for (int c0 = 0; c0 < nv; c0 += chunk) {
+            const int c1 = min(nv, c0 + chunk);
+            if (c0 > 0 && !greedy) {
+                // a counter holds less than 2^15 after a fold, so the logits up to the next cannot overflow it
+                __syncthreads();
+                for (int i = tid; i < kHistBytes / 16; i += kHThreads) {
+                    uint4 v = reinterpret_cast<uint4*>(hist)[i];
+                    if ((v.x | v.y | v.z | v.w) & 0x80008000u) {
+                        uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int q = 0; q < U; ++q)
-                if (i0 + q * kHThreads < nv) v[q] = vec[i0 + q * kHThreads];
+                        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int q = 0; q < U; ++q) {
-                const int i = i0 + q * kHThreads;
-                if (i >= nv) break;
-                const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    word(w[j]);
-                    if (all) {
-                        if (head + 8 * i + 2 * j > 0) count(w[j] & 0xffffu);
-                        count(w[j] >> 16);
+                            for (int h = 0; h < 2; ++h)
+                                if (x[j] & (0x8000u << (16 * h))) {
+                                    x[j] &= ~(0x8000u << (16 * h));
+                                    sh.big[atomicAdd(&sh.n_big, 1u) & (kMaxBig - 1)] = 8 * i + 2 * j + h;
+                                }
+                        reinterpret_cast<uint4*>(hist)[i] = make_uint4(x[0], x[1], x[2], x[3]);
                     }
+                }
+                __syncthreads();
+            }
+            for (int i0 = c0 + tid; i0 < c1; i0 += U * kHThreads) {
+                uint4 v[U];
+#pragma unroll
+                for (int q = 0; q < U; ++q)
+                    if (i0 + q * kHThreads < c1) v[q] = vec[i0 + q * kHThreads];
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    if (i0 + q * kHThreads >= c1) break;
+                    word(v[q].x);
+                    word(v[q].y);
+                    word(v[q].z);
+                    word(v[q].w);
                 }
             }
         }
-        for (int i = tid; i < n - 8 * nv; i += kHThreads) {  // what the vectors leave at both ends
-            const int at = i < head ? i : tail + i - head;
-            const uint32_t raw = raw16[at];
-            word(raw | raw << 16);
-            if (all && at > 0) count(raw);
+        for (int i = tid; i < n - 8 * nv; i += kHThreads) {  // the up to 14 that the vectors leave at both ends
+            const uint32_t raw = raw16[i < head ? i : tail + i - head];
+            const uint32_t w = raw | raw << 16;
+            mx = __hmax2(mx, *reinterpret_cast<const __nv_bfloat162*>(&w));
+            if (!greedy) add((raw << 1) & 0x1fffcu, (raw & 1u) * 65535u + 1u);
         }
         float m = fmaxf(__low2float(mx), __high2float(mx));
         m = warp_max(m);
@@ -567,15 +599,24 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
         __syncthreads();
         if (warp == 0) {
             m = warp_max(__uint_as_float(sh.red32[lane]));
-            if (lane == 0) {
-                sh.maxv = m;
-                sh.first_raw = n > 0 ? raw16[0] : 0x10000u;
-            }
+            if (lane == 0) sh.maxv = m;
         }
+        // groups with a count: a warp looks at eight at a time
+        if (!greedy)
+            for (int i = warp; i < kGroups / 8; i += kHWarps) {
+                const uint4 v = reinterpret_cast<const uint4*>(hist)[32 * i + lane];
+                uint32_t any = __ballot_sync(0xffffffffu, (v.x | v.y | v.z | v.w) != 0);
+                any |= any >> 1;
+                any |= any >> 2;  // bit 4 j: lanes 4 j .. 4 j + 3, the 32 values from 256 i + 32 j on
+                uint32_t bits = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) bits |= ((any >> (4 * j)) & 1u) << j;
+                if (lane == 0) reinterpret_cast<uint8_t*>(sh.map)[i] = static_cast<uint8_t>(bits);
+            }
     }
     cl_sync();
     float M = -INFINITY;
-    for (uint32_t r = 0; r < nc; ++r) M = fmaxf(M, __uint_as_float(cl_ld32(cl_map(&sh.maxv, r))));
+    for (uint32_t r = 0; r < NC; ++r) M = fmaxf(M, __uint_as_float(cl_ld32(cl_map(&sh.maxv, r))));
     M += 0.f;  // -0 counts as +0
     if (M == -INFINITY) {
         if (rank == 0 && tid == 0) {
@@ -589,42 +630,78 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
     uint32_t cut = place_of(__float_as_uint(M) >> 16), ties_kept = 1, kept = 1;
     u64 total = 1ull << kFrac;
     if (!greedy) {
-        // ---- weight and count of every ordered group; the cluster's CTAs take them in turn. A count is
-        // that of all slices and their first logits.
-        uint32_t firsts[kMaxCluster];
+        // ---- weight and count of every group of 32 ordered values in which some CTA has a count; the
+        // cluster's CTAs take those groups in turn
+        uint32_t remote[NC];
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) firsts[r] = r < static_cast<int>(nc) ? cl_ld32(cl_map(&sh.first_raw, r)) : 0x10000u;
-        uint32_t remote[kMaxCluster];
+        for (int r = 0; r < NC; ++r) remote[r] = cl_map(hist, r);
+        uint32_t bigs = 0;  // of all CTAs
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) remote[r] = cl_map(hist, r < static_cast<int>(nc) ? r : 0);
-        // the count of place o; NaN and -inf have no weight and count as 0 here, -0 is part of +0
+        for (int r = 0; r < NC; ++r) bigs += cl_ld32(cl_map(&sh.n_big, r));
         auto count_at = [&](uint32_t raw) {
-            uint32_t s = 0;
+            uint32_t w[NC], s = 0;
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r)
-                if (r < static_cast<int>(nc)) {
-                    const uint32_t w = cl_ld32(remote[r] + ((raw >> 1) << 2));
-                    s += (raw & 1u ? w >> 16 : w & 0xffffu) + (firsts[r] == raw ? 1u : 0u);
-                }
+            for (int r = 0; r < NC; ++r) w[r] = cl_ld32(remote[r] + ((raw << 1) & 0x1fffcu));
+#pragma unroll
+            for (int r = 0; r < NC; ++r) s += raw & 1u ? w[r] >> 16 : w[r] & 0xffffu;
+            if (bigs)
+                for (int r = 0; r < NC; ++r)
+                    for (uint32_t b = 0; b < cl_ld32(cl_map(&sh.n_big, r)); ++b)
+                        if (cl_ld32(cl_map(&sh.big[b], r)) == raw) s += kFold;
             return s;
         };
+        // the count of place o; NaN and -inf have no weight and count as 0 here, -0 is part of +0
         auto place_count = [&](uint32_t o) -> uint32_t {
             if (is_nan_place(o) || o == kPlaceNegZero || o == kPlaceNegInf) return 0;
             return count_at(raw_of(o)) + (o == kPlaceZero ? count_at(0x8000u) : 0u);
         };
-        const uint32_t mass_at = cl_map(sh.mass, 0), cnt_at = cl_map(sh.cnt, 0);
-        for (int g = rank + nc * warp; g < kGroups; g += nc * kHWarps) {
-            const uint32_t o = 32 * g + lane;
-            uint32_t cn = place_count(o);
-            u64 ms = 0;
-            if (__any_sync(0xffffffffu, cn != 0)) {
-                if (cn) ms = cn * weight(value_at(o), M, c, sh.table);
-#pragma unroll
-                for (int q = 16; q; q >>= 1) {
-                    cn += __shfl_xor_sync(0xffffffffu, cn, q);
-                    ms += __shfl_xor_sync(0xffffffffu, ms, q);
-                }
+        if (rank == 0)
+            for (int g = tid; g < kGroups; g += kHThreads) {
+                sh.mass[g] = 0;
+                sh.cnt[g] = 0;
             }
+        if (warp == 0) {
+            // the groups of raw values with a count, as places: 32 neighbours are neighbours there too
+            uint32_t m[2] = {0, 0};
+#pragma unroll
+            for (int r = 0; r < NC; ++r) {
+                m[0] |= cl_ld32(cl_map(&sh.map[2 * lane], r));
+                m[1] |= cl_ld32(cl_map(&sh.map[2 * lane + 1], r));
+            }
+            // folded counters may have emptied their group
+            for (int r = 0; r < NC && bigs; ++r)
+                for (uint32_t b = 0; b < cl_ld32(cl_map(&sh.n_big, r)); ++b) {
+                    const uint32_t g = cl_ld32(cl_map(&sh.big[b], r)) >> 5;
+                    if (g >> 6 == static_cast<uint32_t>(lane)) m[(g >> 5) & 1] |= 1u << (g & 31);
+                }
+            // -0 (raw 0x8000, group 1024, word 32) counts at +0's place (group 0)
+            const uint32_t neg = __shfl_sync(0xffffffffu, m[0], 16) & 1u;
+            if (lane == 0) m[0] |= neg;
+            int at = __popc(m[0]) + __popc(m[1]), all = at;
+#pragma unroll
+            for (int q = 1; q < 32; q <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, at, q);
+                if (lane >= q) at += x;
+            }
+            if (lane == 31) sh.n_list = at;
+            at -= all;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                while (m[h]) {
+                    const uint32_t g = 32 * (2 * lane + h) + __ffs(m[h]) - 1;
+                    m[h] &= m[h] - 1;
+                    sh.list[at++] = static_cast<uint16_t>(place_of(32 * g) >> 5);
+                }
+        }
+        cl_sync();  // and the first CTA's sums are cleared
+        const uint32_t mass_at = cl_map(sh.mass, 0), cnt_at = cl_map(sh.cnt, 0);
+        for (uint32_t i = rank + NC * warp; i < sh.n_list; i += NC * kHWarps) {
+            const uint32_t g = sh.list[i], o = 32 * g + lane;
+            uint32_t cn = place_count(o);
+            u64 ms = cn ? cn * weight(value_at(o), M, c, sh.table) : 0;
+            cn = __reduce_add_sync(0xffffffffu, cn);
+#pragma unroll
+            for (int q = 16; q; q >>= 1) ms += __shfl_xor_sync(0xffffffffu, ms, q);
             if (lane == 0) {
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mass_at + 8 * g), "l"(ms) : "memory");
                 asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cnt_at + 4 * g), "r"(cn) : "memory");
@@ -782,18 +859,14 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
                     const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
                     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
                     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-                    if (!__hbge2(cut2, m) || ties_kept) {
-                        // some logit lies above the cut (or may lie at it)
-                        const float ma = fmaxf(__low2float(m), __high2float(m));
-                        if (ma >= cut_v)
+                    if (__hblt2(m, cut2)) continue;  // all eight lie below the cut
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                bool tie;
-                                sum += look(canon(__uint_as_float(w[j] << 16)), tie);
-                                ties += tie;
-                                sum += look(canon(__uint_as_float(w[j] & 0xffff0000u)), tie);
-                                ties += tie;
-                            }
+                    for (int j = 0; j < 4; ++j) {
+                        bool tie;
+                        sum += look(canon(__uint_as_float(w[j] << 16)), tie);
+                        ties += tie;
+                        sum += look(canon(__uint_as_float(w[j] & 0xffff0000u)), tie);
+                        ties += tie;
                     }
                 }
             }
@@ -888,14 +961,25 @@ void launch_cluster(void (*kern)(P...), int rows, int nc, int threads, size_t sm
     HYB_LAUNCH_CHECK("sample_batch kernel");
 }
 
+template <int NC>
+void launch_hist_t(const SampleBatchParams& p, cudaStream_t stream) {
+    const int slice = ((p.vocab + NC - 1) / NC + 7) & ~7;
+    allow_smem(reinterpret_cast<const void*>(sample_hist_kernel<NC>), kHistBytes + sizeof(HShare));
+    launch_cluster(sample_hist_kernel<NC>, p.rows, NC, kHThreads, kHistBytes + sizeof(HShare), stream, p, slice);
+}
+
 void launch_hist(const SampleBatchParams& p, cudaStream_t stream) {
-    // the fewest CTAs a row whose slices fit the counters; more while the rows alone leave SMs idle
+    // the fewest CTAs a row whose slices fit; more while all rows stay resident at once (one CTA an
+    // SM) and a slice is worth one
     int nc = 1;
     while (nc < kMaxCluster && (p.vocab + nc - 1) / nc > kHSlice) nc *= 2;
     while (nc < kMaxCluster && p.rows * nc * 2 <= num_sms() && p.vocab / nc >= 8192) nc *= 2;
-    const int slice = ((p.vocab + nc - 1) / nc + 7) & ~7;
-    allow_smem(reinterpret_cast<const void*>(sample_hist_kernel), kHistBytes + sizeof(HShare));
-    launch_cluster(sample_hist_kernel, p.rows, nc, kHThreads, kHistBytes + sizeof(HShare), stream, p, slice);
+    switch (nc) {
+        case 1: launch_hist_t<1>(p, stream); break;
+        case 2: launch_hist_t<2>(p, stream); break;
+        case 4: launch_hist_t<4>(p, stream); break;
+        default: launch_hist_t<8>(p, stream); break;
+    }
 }
 
 void launch_f32(const SampleBatchParams& p, cudaStream_t stream) {

@@ -555,6 +555,29 @@ def test_sample_batch_edges(built_lib, V):
         run_sample(x, u, t, k, p, mp, torch.bfloat16)
 
 
+@pytest.mark.parametrize("V,offset", [(131072, 0), (131063, 3)])
+def test_sample_batch_values_that_repeat(built_lib, V, offset):
+    """A value that fills a whole slice of the row, and ones that fill halves and quarters of it."""
+    import torch
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((80, V)).astype(np.float32)
+    x[0] = 0.5
+    x[1] = -2.0
+    x[1, 7] = 1.0
+    x[2] = np.where(np.arange(V) % 2, 3.0, 2.0)
+    x[3] = np.where(np.arange(V) < 70000, 1.5, -1.5)
+    x[4] = np.where(np.arange(V) % 4, 0.0, -0.0)
+    x[5] = np.repeat(np.float32([1, 2, 3, 4]), V // 4 + 1)[:V]
+    x[6, : V // 2] = -np.inf
+    x[7, 5000:] = np.nan
+    t = np.resize([1.0, 0.6, 0.0], 80)
+    k = np.resize([0, 50000, 0, 100000, 3], 80)
+    p = np.resize([0.0, 0.9, 0.0, 0.5], 80)
+    mp = np.resize([0.0, 0.0, 0.0, 0.0, 0.0, 0.3], 80)
+    run_sample(x, rng.random(80, dtype=np.float32), t, k, p, mp, torch.bfloat16, pad=offset, offset=offset)
+    run_sample(x[:8], rng.random(8, dtype=np.float32), 1.0, 0, 0.7, 0.0, torch.bfloat16)
+
+
 def test_sample_batch_defaults_and_strange_settings(built_lib):
     import torch
     from hyperion_b200 import ops

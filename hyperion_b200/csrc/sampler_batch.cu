@@ -9,10 +9,8 @@
 // T <= 0 takes the first maximum.
 //
 // Exactness. Sums decide which token is drawn, so they must not depend on the order of the
-// additions: weights are integers, w = rint(exp(..) * 2^44), and their 64-bit sums are exact
-// in any order (vocabulary <= 2^19). exp is evaluated in double as 2^d, d = (x - M) log2(e) / T:
-// d = n/32 + r with |r| <= 1/64, 2^r by its Taylor polynomial of degree 5 in r ln 2 (the next
-// term is below (ln 2 / 64)^6 / 720 = 2e-15), 2^(j/32) from a 32-entry table.
+// additions: weights are 44-bit integers (Weight below), and their 64-bit sums are exact in any
+// order (vocabulary <= 2^19).
 //
 // One thread-block cluster per row; CTA c of the cluster owns a contiguous slice of the row.
 //
@@ -45,6 +43,7 @@ constexpr int kWarpsS = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kFrac = 44;
 constexpr int kMaxCluster = 8;
+constexpr int kTableCopies = 16;  // of the table of powers: the lanes of a half-warp read 16 bank pairs
 constexpr int kSliceBytes = 128 * 1024;  // the largest slice held in shared memory
 // A slice has at most 2^19 / 8 = 65536 logits, so its limb sums fit 32 bits: 65535 * 65536 < 2^32.
 
@@ -72,7 +71,7 @@ struct Share {  // read by the other CTAs of the cluster
     uint32_t wties[kWarpsS];
     u64 red[kWarpsS];
     uint32_t red32[kWarpsS];
-    double table[32];
+    u64 table[32 * kTableCopies];
 };
 
 __device__ __forceinline__ void cl_sync() {
@@ -118,25 +117,55 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-// rint(2^44 * exp((x - M) / T)), c = log2(e) / T.
-__device__ __forceinline__ u64 weight(float x, float M, double c, const double* table) {
-    if (x == M) return 1ull << kFrac;
-    const double d = (static_cast<double>(x) - static_cast<double>(M)) * c;
-    if (!(d > -(kFrac + 2.0))) return 0;
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
-    const double t = fma(d, 32.0, kMagic);
-    const int n = __double2loint(t);
-    const double r = fma(t - kMagic, -1.0 / 32.0, d) * 0.69314718055994530942;
-    double q = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    q = fma(q, r, 1.0 / 6.0);
-    q = fma(q, r, 0.5);
-    q = fma(q, r, 1.0);
-    q = fma(q, r, 1.0);
-    const double v = q * table[n & 31];
-    // times 2^(n >> 5) 2^44 by the exponent field (results from 2^-2 up), then rounded to an integer
-    const double s = __hiloint2double(__double2hiint(v) + ((n >> 5) + kFrac) * (1 << 20), __double2loint(v));
-    return static_cast<u64>(__double_as_longlong(s + 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-}
+// 2^44 * exp((x - M) / T) as an integer, without a branch on x, in fp32 pairs and integers (in
+// double the same steps take over twice as long: an SM has a quarter as many lanes for it).
+// d = (x - M) log2(e) / T as a pair: x - M exactly as s + e, the factor as c + cl, the product's error
+// by a fused multiply-add. d = n/32 + r; 2^(n/32) is a 44-bit table entry shifted, and the entry's
+// (2^r - 1) share, |r| <= 1/64, is an fp32 polynomial's, added in units of 2^17. Off by at most
+// some 2^-27 of the weight, at random; far below what moves a draw between two tokens (the sums
+// of thousands of weights average it further).
+struct Weight {
+    float M, c, cl;
+    uint32_t table;  // of this lane
+    bool inf;        // the maximum is +inf: its tokens share all the weight
+    __device__ __forceinline__ Weight(float max, float temperature, const u64* t) : M(max), inf(max == INFINITY) {
+        const double f = 1.4426950408889634074 / static_cast<double>(temperature);
+        c = static_cast<float>(fmin(f, 3e38));
+        cl = f < 3e38 ? static_cast<float>(f - static_cast<double>(c)) : 0.f;
+        table = smem_u32(t) + (threadIdx.x & (kTableCopies - 1)) * 8;
+    }
+    // thread t < 32 fills its entry
+    static __device__ __forceinline__ void fill(u64* t) {
+        const u64 v = static_cast<u64>(rint(exp2(threadIdx.x * (1.0 / 32.0)) * 17592186044416.0));
+        for (int i = 0; i < kTableCopies; ++i) t[threadIdx.x * kTableCopies + i] = v;
+    }
+    __device__ __forceinline__ u64 operator()(float x) const {
+        if (inf) return x == INFINITY ? 1ull << kFrac : 0;
+        const float s = x - M, bb = s - x, e = (x - (s - bb)) - (M + bb);  // two-sum of x and -M
+        float d = s * c;
+        float dl = fmaf(s, c, -d);
+        dl = fmaf(s, cl, dl);
+        dl = fmaf(e, c, dl);
+        const bool some = d > -60.f;  // below, at -inf and for NaN the weight is 0
+        d = some ? d : -60.f;
+        constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+        const float t = fmaf(d, 32.f, kMagic);
+        const int n = __float_as_int(t) - __float_as_int(kMagic);
+        const float r = fmaf(t - kMagic, -1.f / 32.f, d) + (some ? dl : 0.f);
+        float q = fmaf(r, 9.6181291e-3f, 5.5504109e-2f);
+        q = fmaf(q, r, 0.24022651f);
+        q = fmaf(q, r, 0.69314718f);
+        q *= r;  // 2^r - 1
+        u64 v;
+        asm("ld.shared.u64 %0, [%1];" : "=l"(v) : "r"(table + (n & 31) * (kTableCopies * 8)));
+        // v 2^-17 as a float by its upper bits: 2^44 <= v < 2^45
+        const float vf = __uint_as_float(0x4d000000u | (static_cast<uint32_t>(v >> 21) & 0x7fffffu));
+        const int add = __float_as_int(fmaf(vf, q, kMagic)) - __float_as_int(kMagic);  // |add| < 2^22
+        v += static_cast<long long>(add) * 131072;
+        const int k = -(n >> 5);
+        return some ? (v + ((1ull << k) >> 1)) >> k : 0;
+    }
+};
 
 // Inclusive block scan in thread order; *total is the block's sum.
 template <typename V>
@@ -178,8 +207,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
     int k = p.top_k ? p.top_k[row] : 0;
     float tp = p.top_p ? p.top_p[row] : 0.f, mp = p.min_p ? p.min_p[row] : 0.f;
     const bool use_k = k > 0 && k < p.vocab, use_p = tp > 0.f && tp < 1.f, use_m = mp > 0.f;
-    const double c = 1.4426950408889634074 / static_cast<double>(temp);
-    if (tid < 32) sh.table[tid] = exp2(tid * (1.0 / 32.0));
+    if (tid < 32) Weight::fill(sh.table);
 
     // ---- the slice into shared memory, its maximum (first index)
     u64 best = 0;
@@ -226,6 +254,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
     const uint32_t arg = ~static_cast<uint32_t>(best);
     const float M = value_of(static_cast<uint32_t>(best >> 32));
     const float* x = resident ? buf : gx;
+    const Weight weight(M, temp, sh.table);
     const bool empty = M == -INFINITY;
     if (greedy || empty) {
         if (rank == 0 && tid == 0) {
@@ -258,7 +287,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
                 const uint32_t bin = (key >> shift) & ((1u << width) - 1);
                 atomicAdd(&h.cnt[bin], 1u);
                 if (use_p) {
-                    const u64 w = weight(xi, M, c, sh.table);
+                    const u64 w = weight(xi);
                     if (w) {
                         atomicAdd(&h.l0[bin], static_cast<uint32_t>(w) & 0xffffu);
                         if (w >> 16) atomicAdd(&h.l1[bin], static_cast<uint32_t>(w >> 16) & 0xffffu);
@@ -315,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
         uint32_t take = in_bin;
         if (use_k) take = min(take, static_cast<uint32_t>(k) - above);
         if (use_p) {
-            const u64 w = weight(value_of(cut_key), M, c, sh.table);
+            const u64 w = weight(value_of(cut_key));
             if (w) take = static_cast<uint32_t>(min(static_cast<u64>(take), (target - mass_above + w - 1) / w));
         }
         ties_kept = take;
@@ -336,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
                 ties += key == cut_key;
                 continue;
             }
-            const u64 w = weight(xi, M, c, sh.table);
+            const u64 w = weight(xi);
             if (passes(w)) {
                 sum += w;
                 ++cnt;
@@ -368,7 +397,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
         }
     }
     cl_sync();
-    u64 tie_w = cut ? weight(value_of(cut_key), M, c, sh.table) : 0;
+    u64 tie_w = cut ? weight(value_of(cut_key)) : 0;
     if (cut && !passes(tie_w)) {
         tie_w = 0;
         ties_kept = 0;
@@ -417,7 +446,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
         const uint32_t key = key_of(xi);
         tie = cut && key == cut_key;
         if (cut && key <= cut_key) return 0;
-        const u64 w = weight(xi, M, c, sh.table);
+        const u64 w = weight(xi);
         return passes(w) ? w : 0;
     };
     for (int i = i0; i < i1; ++i) {
@@ -455,6 +484,9 @@ constexpr int kHistBytes = 65536 * 2;
 constexpr int kHSlice = 131072;
 constexpr int kFold = 32768;           // logits between two folds of the counters
 constexpr int kMaxBig = kHSlice / kFold;
+constexpr int kBinades = 16;           // of the table of weights by value, either sign
+constexpr int kHalfTab = kBinades * 128;
+constexpr uint32_t kManyKept = 1024;   // kept tokens from which the table pays
 
 // Values in descending order: place o in [0, 65536) <-> raw bits. Positive ones (NaNs above +inf
 // first, whose counts are moved to -inf), then negative ones; -0 (0x8000) has the place after +0.
@@ -465,8 +497,11 @@ __device__ __forceinline__ bool is_nan_place(uint32_t o) { return (raw_of(o) & 0
 __device__ __forceinline__ float value_at(uint32_t o) { return __uint_as_float(raw_of(o) << 16); }
 
 struct HShare {
-    double table[32];
-    u64 mass[kGroups];       // (first CTA) weight of a group
+    u64 table[32 * kTableCopies];
+    union {
+        u64 mass[kGroups];       // (first CTA) weight of a group
+        u64 by_value[2 * kHalfTab];  // later: the weights of the values in the upper binades
+    };
     uint32_t cnt[kGroups];   // (first CTA) its count
     u64 red[kHWarps];
     uint32_t red32[kHWarps];
@@ -475,6 +510,8 @@ struct HShare {
     uint32_t big[kMaxBig];   // .. each stands for 2^15 logits of this value more
     uint32_t map[kGroups / 32];  // groups with a count
     uint32_t n_list;
+    float row_max;
+    uint32_t bigs;           // folded counters of all CTAs
     uint16_t list[kGroups];      // the groups in which some CTA has a count
     uint32_t cut, ties;      // (first CTA) the last kept value's place, how many of it are kept
     uint32_t kept;
@@ -527,10 +564,9 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
     const int k = p.top_k ? p.top_k[row] : 0;
     const float tp = p.top_p ? p.top_p[row] : 0.f, mp = p.min_p ? p.min_p[row] : 0.f, u = p.u[row];
     const bool use_k = k > 0 && k < p.vocab, use_p = tp > 0.f && tp < 1.f, use_m = mp > 0.f;
-    const double c = 1.4426950408889634074 / static_cast<double>(temp);
 
     for (int i = tid; i < kHistBytes / 16; i += kHThreads) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
-    if (tid < 32) sh.table[tid] = exp2(tid * (1.0 / 32.0));
+    if (tid < 32) Weight::fill(sh.table);
     if (tid == 0) sh.n_big = 0;
     __syncthreads();
 
@@ -615,29 +651,78 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
             }
     }
     cl_sync();
-    float M = -INFINITY;
-    for (uint32_t r = 0; r < NC; ++r) M = fmaxf(M, __uint_as_float(cl_ld32(cl_map(&sh.maxv, r))));
-    M += 0.f;  // -0 counts as +0
+    // ---- the first warp gathers what the others found (a few remote loads, each once a CTA): the
+    // row's maximum, the folded counters and the groups in which some CTA has a count
+    if (warp == 0) {
+        float m = lane < NC ? __uint_as_float(cl_ld32(cl_map(&sh.maxv, lane))) : -INFINITY;
+        m = warp_max(m) + 0.f;  // -0 counts as +0
+        uint32_t big = lane < NC ? cl_ld32(cl_map(&sh.n_big, lane)) : 0;
+        const uint32_t bigs = __reduce_add_sync(0xffffffffu, big);
+        if (!greedy) {
+            uint32_t g2[2] = {0, 0}, w[2][NC];
+#pragma unroll
+            for (int r = 0; r < NC; ++r) {
+                w[0][r] = cl_ld32(cl_map(&sh.map[2 * lane], r));
+                w[1][r] = cl_ld32(cl_map(&sh.map[2 * lane + 1], r));
+            }
+#pragma unroll
+            for (int r = 0; r < NC; ++r) {
+                g2[0] |= w[0][r];
+                g2[1] |= w[1][r];
+            }
+            if (bigs)
+                for (int r = 0; r < NC; ++r)
+                    for (uint32_t b = 0; b < __shfl_sync(0xffffffffu, big, r); ++b) {
+                        // a fold may have emptied the counter's group
+                        const uint32_t g = cl_ld32(cl_map(&sh.big[b], r)) >> 5;
+                        if (g >> 6 == static_cast<uint32_t>(lane)) g2[(g >> 5) & 1] |= 1u << (g & 31);
+                    }
+            // -0 (raw 0x8000, group 1024, word 32) counts at +0's place (group 0)
+            const uint32_t neg = __shfl_sync(0xffffffffu, g2[0], 16) & 1u;
+            if (lane == 0) g2[0] |= neg;
+            uint32_t at = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                for (uint32_t left = __ballot_sync(0xffffffffu, g2[h] != 0); left; left &= left - 1) {
+                    const int src = __ffs(left) - 1;
+                    const uint32_t bits = __shfl_sync(0xffffffffu, g2[h], src);
+                    const uint32_t g = 32 * (2 * src + h) + lane;
+                    if (bits >> lane & 1u)  // 32 neighbouring raw values are 32 neighbouring places
+                        sh.list[at + __popc(bits & ((1u << lane) - 1))] = static_cast<uint16_t>(place_of(32 * g) >> 5);
+                    at += __popc(bits);
+                }
+            if (lane == 0) sh.n_list = at;
+        }
+        if (lane == 0) {
+            sh.row_max = m;
+            sh.bigs = bigs;
+        }
+    } else if (rank == 0) {
+        for (int g = tid - 32; g < kGroups; g += kHThreads - 32) {
+            sh.mass[g] = 0;
+            sh.cnt[g] = 0;
+        }
+    }
+    cl_sync();  // the first CTA's sums are cleared
+    const float M = sh.row_max;
     if (M == -INFINITY) {
         if (rank == 0 && tid == 0) {
             p.token[row] = -1;
             if (p.kept) p.kept[row] = 0;
             if (p.prob) p.prob[row] = 0.f;
         }
-        cl_sync();  // no CTA leaves while another may read its shared memory
-        return;
+        return;  // no CTA reads another's shared memory from here on
     }
+    const Weight weight(M, greedy ? 1.f : temp, sh.table);
     uint32_t cut = place_of(__float_as_uint(M) >> 16), ties_kept = 1, kept = 1;
     u64 total = 1ull << kFrac;
     if (!greedy) {
-        // ---- weight and count of every group of 32 ordered values in which some CTA has a count; the
-        // cluster's CTAs take those groups in turn
+        // ---- weight and count of every listed group of 32 ordered values; the cluster's CTAs take them in
+        // turn
         uint32_t remote[NC];
 #pragma unroll
         for (int r = 0; r < NC; ++r) remote[r] = cl_map(hist, r);
-        uint32_t bigs = 0;  // of all CTAs
-#pragma unroll
-        for (int r = 0; r < NC; ++r) bigs += cl_ld32(cl_map(&sh.n_big, r));
+        const uint32_t bigs = sh.bigs;
         auto count_at = [&](uint32_t raw) {
             uint32_t w[NC], s = 0;
 #pragma unroll
@@ -655,50 +740,11 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
             if (is_nan_place(o) || o == kPlaceNegZero || o == kPlaceNegInf) return 0;
             return count_at(raw_of(o)) + (o == kPlaceZero ? count_at(0x8000u) : 0u);
         };
-        if (rank == 0)
-            for (int g = tid; g < kGroups; g += kHThreads) {
-                sh.mass[g] = 0;
-                sh.cnt[g] = 0;
-            }
-        if (warp == 0) {
-            // the groups of raw values with a count, as places: 32 neighbours are neighbours there too
-            uint32_t m[2] = {0, 0};
-#pragma unroll
-            for (int r = 0; r < NC; ++r) {
-                m[0] |= cl_ld32(cl_map(&sh.map[2 * lane], r));
-                m[1] |= cl_ld32(cl_map(&sh.map[2 * lane + 1], r));
-            }
-            // folded counters may have emptied their group
-            for (int r = 0; r < NC && bigs; ++r)
-                for (uint32_t b = 0; b < cl_ld32(cl_map(&sh.n_big, r)); ++b) {
-                    const uint32_t g = cl_ld32(cl_map(&sh.big[b], r)) >> 5;
-                    if (g >> 6 == static_cast<uint32_t>(lane)) m[(g >> 5) & 1] |= 1u << (g & 31);
-                }
-            // -0 (raw 0x8000, group 1024, word 32) counts at +0's place (group 0)
-            const uint32_t neg = __shfl_sync(0xffffffffu, m[0], 16) & 1u;
-            if (lane == 0) m[0] |= neg;
-            int at = __popc(m[0]) + __popc(m[1]), all = at;
-#pragma unroll
-            for (int q = 1; q < 32; q <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, at, q);
-                if (lane >= q) at += x;
-            }
-            if (lane == 31) sh.n_list = at;
-            at -= all;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                while (m[h]) {
-                    const uint32_t g = 32 * (2 * lane + h) + __ffs(m[h]) - 1;
-                    m[h] &= m[h] - 1;
-                    sh.list[at++] = static_cast<uint16_t>(place_of(32 * g) >> 5);
-                }
-        }
-        cl_sync();  // and the first CTA's sums are cleared
         const uint32_t mass_at = cl_map(sh.mass, 0), cnt_at = cl_map(sh.cnt, 0);
         for (uint32_t i = rank + NC * warp; i < sh.n_list; i += NC * kHWarps) {
             const uint32_t g = sh.list[i], o = 32 * g + lane;
             uint32_t cn = place_count(o);
-            u64 ms = cn ? cn * weight(value_at(o), M, c, sh.table) : 0;
+            u64 ms = cn ? cn * weight(value_at(o)) : 0;
             cn = __reduce_add_sync(0xffffffffu, cn);
 #pragma unroll
             for (int q = 16; q; q >>= 1) ms += __shfl_xor_sync(0xffffffffu, ms, q);
@@ -740,7 +786,7 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
             if (any_cut && warp == 0) {
                 const uint32_t o = 32 * sh.red32[0] + lane;
                 const uint32_t cn = place_count(o);
-                const u64 w = cn ? weight(value_at(o), M, c, sh.table) : 0, ms = cn * w;
+                const u64 w = cn ? weight(value_at(o)) : 0, ms = cn * w;
                 uint32_t ci = cn;
                 u64 mi = ms;
 #pragma unroll
@@ -769,19 +815,27 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
                 // min-p: the kept tokens with w >= min_p; where the cut's own weight passes nothing changes
                 const double mpd = static_cast<double>(fminf(mp, 1.f)) * 17592186044416.0;
                 const uint32_t kc = sh.cut;
-                const bool cut_passes = kc < 65536u && static_cast<double>(weight(value_at(kc), M, c, sh.table)) >= mpd;
+                const bool cut_passes = kc < 65536u && static_cast<double>(weight(value_at(kc))) >= mpd;
                 if (!cut_passes) {
                     // weights fall along the places, so the passing places are a prefix, which ends before the
-                    // cut: a binary search by one thread over all 65536, then the sums of the groups before
-                    uint32_t a = 0, b = min(kc, 65536u);  // places < a pass, places >= b do not
-                    while (a < b) {
-                        const uint32_t mid = (a + b) >> 1;
-                        const float x = is_nan_place(mid) ? (mid < 32768u ? INFINITY : -INFINITY) : value_at(mid);
-                        const bool pass = x >= M || static_cast<double>(weight(x, M, c, sh.table)) >= mpd;
-                        if (pass) a = mid + 1;
-                        else b = mid;
+                    // cut: near M + T ln(min_p), found there by 32 places at a time
+                    const float guess = M + temp * logf(fminf(mp, 1.f));
+                    int first = static_cast<int>(place_of(__bfloat16_as_ushort(f2bf(guess)))) - 16;
+                    uint32_t end = 0;
+                    for (int way = 0;;) {  // up or down, never back
+                        first = max(0, min(first, 65536 - 32));
+                        const uint32_t o = first + lane;
+                        const float x = is_nan_place(o) ? (o < 32768u ? INFINITY : -INFINITY) : value_at(o);
+                        const bool pass = x >= M || static_cast<double>(weight(x)) >= mpd;
+                        const int passing = __popc(__ballot_sync(0xffffffffu, pass));
+                        end = first + passing;
+                        if (passing == 32 && first < 65536 - 32 && way >= 0) way = 1;
+                        else if (passing == 0 && first > 0 && way <= 0) way = -1;
+                        else break;
+                        first += 32 * way;
                     }
-                    const uint32_t end = a, ge = end >> 5;
+                    end = min(end, kc);
+                    const uint32_t ge = end >> 5;
                     __syncthreads();
                     if (2 * tid <= ge && ge <= 2 * tid + 1) {
                         const bool second = ge == 2u * tid + 1;
@@ -795,7 +849,7 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
                         const uint32_t o = 32 * ge + lane;
                         if (o < end) {
                             cn = place_count(o);
-                            ms = cn ? cn * weight(value_at(o), M, c, sh.table) : 0;
+                            ms = cn ? cn * weight(value_at(o)) : 0;
                         }
 #pragma unroll
                         for (int q = 16; q; q >>= 1) {
@@ -823,13 +877,28 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
 
     // ---- second pass: kept weight of every warp's run of the slice, in index order
     const float cut_v = cut < 65536u ? (is_nan_place(cut) ? (cut < 32768u ? INFINITY : -INFINITY) : value_at(cut) + 0.f) : -INFINITY;
-    const u64 tie_w = ties_kept ? weight(cut_v, M, c, sh.table) : 0;
+    const u64 tie_w = ties_kept ? weight(cut_v) : 0;
     // above: places before the cut. Without a cut everything above -inf is (weight 0 below).
     auto look = [&](float x, bool& tie) -> u64 {
         tie = ties_kept && x == cut_v;
-        return x > cut_v ? weight(x, M, c, sh.table) : 0;
+        return x > cut_v ? weight(x) : 0;
     };
     const int run = ((slice + kHWarps - 1) / kHWarps + 255) & ~255;  // whole warp-wide vectors
+    // with many tokens kept, the weights of all values in 16 binades below the largest magnitude that
+    // has a weight are tabulated (four a thread) and looked up
+    const bool many = kept > kManyKept && !weight.inf;
+    uint32_t tab_base = 0;
+    if (many) {
+        const float far = fmaxf(fabsf(M), fabsf(M - 42.f * temp));  // exp(-42) is below 2^-60
+        tab_base = static_cast<uint32_t>(max(0, static_cast<int>(min(__float_as_uint(far) >> 23, 254u)) - kBinades + 1)) << 7;
+        for (int i = tid; i < 2 * kHalfTab; i += kHThreads) {
+            const float x = canon(__uint_as_float((tab_base + (i & (kHalfTab - 1)) | (i >= kHalfTab ? 0x8000u : 0u)) << 16));
+            bool tie;
+            const u64 w = look(x, tie);
+            sh.by_value[i] = tie ? 1ull << 52 : w;
+        }
+        __syncthreads();
+    }
     {
         const int from = warp * run, to = min(n, from + run);  // vectors and ends, counted from `head` on
         u64 sum = 0;
@@ -848,25 +917,54 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
             const int a_end = min(to, head + 8 * v0), b_start = max(a_end, head + 8 * v1);
             for (int i = from + lane; i < a_end; i += 32) one(i);
             for (int i = b_start + lane; i < to; i += 32) one(i);
-            for (int i0 = v0 + lane; i0 < v1; i0 += 4 * 32) {
-                uint4 v[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (i0 + 32 * q < v1) v[q] = vec[i0 + 32 * q];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (i0 + 32 * q >= v1) break;
-                    const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-                    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
-                    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-                    if (__hblt2(m, cut2)) continue;  // all eight lie below the cut
+            if (many) {
+                // every logit by one lookup; entry 2^52 stands for a logit at the cut (a thread's weights
+                // stay below 2^52)
+                u64 both = 0;
+                auto add = [&](uint32_t raw) {
+                    const uint32_t at = (raw & 0x7fffu) - tab_base;
+                    if (at < static_cast<uint32_t>(kHalfTab)) {
+                        both += sh.by_value[at + (raw >> 15) * kHalfTab];
+                    } else {
+                        const float x = canon(__uint_as_float(raw << 16));
+                        if (x >= cut_v) {
+                            bool tie;
+                            sum += look(x, tie);
+                            ties += tie;
+                        }
+                    }
+                };
+                uint4 v = v0 + lane < v1 ? vec[v0 + lane] : make_uint4(0, 0, 0, 0);
+                for (int i0 = v0 + lane; i0 < v1; i0 += 32) {
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    if (i0 + 32 < v1) v = vec[i0 + 32];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        bool tie;
-                        sum += look(canon(__uint_as_float(w[j] << 16)), tie);
-                        ties += tie;
-                        sum += look(canon(__uint_as_float(w[j] & 0xffff0000u)), tie);
-                        ties += tie;
+                        add(w[j] & 0xffffu);
+                        add(w[j] >> 16);
+                    }
+                }
+                sum += both & ((1ull << 52) - 1);
+                ties += static_cast<uint32_t>(both >> 52);
+            } else {
+                for (int i0 = v0 + lane; i0 < v1; i0 += 4 * 32) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (i0 + 32 * q < v1) v[q] = vec[i0 + 32 * q];
+                    // vectors with a logit that does not lie below the cut
+                    uint32_t take = 0;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+                        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+                        const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+                        if (i0 + 32 * q < v1 && !__hblt2(m, cut2)) take |= 1u << q;
+                    }
+                    for (; take; take &= take - 1) {
+                        const int at = head + 8 * (i0 + 32 * (__ffs(take) - 1));
+#pragma unroll 1
+                        for (int j = 0; j < 8; ++j) one(at + j);
                     }
                 }
             }

@@ -198,14 +198,14 @@ def _switch(dev, stream):
     """None where the call can go to the current stream as it is; otherwise the context that makes
     its device and stream current, so that what the call allocates belongs to them."""
     if stream is None:
-        return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+        return None if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
     if stream.device.index != dev:
         raise ValueError(f"the stream is on {stream.device}, the tensors on cuda:{dev}")
     return torch.cuda.stream(stream)
 
 
 def _here(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 class PagedPlan:
@@ -214,9 +214,15 @@ class PagedPlan:
     refused, bad pages). Reused from step to step by passing it back as `plan`."""
 
     def __init__(self, n_req: int, max_rows: int, device="cuda"):
-        sizes = [n_req + 1, max_rows, max_rows, max_rows, n_req, 4]
-        parts = torch.empty(sum(sizes), dtype=_I32, device=device).split(sizes)
-        self.row_start, self.row_req, self.row_pos, self.slot_map, self.total_lens, self.status = parts
+        whole = torch.empty(2 * n_req + 3 * max_rows + 5, dtype=_I32, device=device)
+        (self.row_start, self.row_req, self.row_pos, self.slot_map, self.total_lens, self.status) = whole.split_with_sizes(
+            [n_req + 1, max_rows, max_rows, max_rows, n_req, 4])
+        # the parts' addresses, in the order of the C arguments
+        a = whole.data_ptr()
+        b = a + 4 * (n_req + 1)
+        r = 4 * max_rows
+        self._at = (a, b, b + r, b + 2 * r, b + 3 * r, b + 3 * r + 4 * n_req)
+        self._key = (n_req, max_rows, whole.get_device())
 
 
 def paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages: int, page_size: int, max_rows: int, pos0=0,
@@ -234,12 +240,9 @@ def paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages: int, pag
             return paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages, page_size, max_rows, pos0, plan)
     if plan is None:
         plan = PagedPlan(n, max_rows, cached_lens.device)
-    rows = (max_rows,)
-    check(lib().hyb_paged_plan(c, a, n, page_size, n_pages, f, n_free, b, width, pos0, max_rows,
-                               _ck("row_start", plan.row_start, _I32, (n + 1,), dev), _ck("row_req", plan.row_req, _I32, rows, dev),
-                               _ck("row_pos", plan.row_pos, _I32, rows, dev), _ck("slot_map", plan.slot_map, _I32, rows, dev),
-                               _ck("total_lens", plan.total_lens, _I32, (n,), dev), _ck("status", plan.status, _I32, (4,), dev),
-                               _here(dev)))
+    if plan._key != (n, max_rows, dev):
+        raise ValueError(f"plan is for (requests, rows, device) {plan._key}, the call has {(n, max_rows, dev)}")
+    check(lib().hyb_paged_plan(c, a, n, page_size, n_pages, f, n_free, b, width, pos0, max_rows, *plan._at, _here(dev)))
     return plan
 
 
@@ -308,7 +311,7 @@ def sdpa_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len: int, block_t
                                       max_q, max_own, window, scale, softcap, scratch, out)
     L = lib()
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty(shape, dtype=_BF16, device=q.device)
     if scratch is None:
         scratch = SharedPrefixScratch(T, n, max_q, max_own, prefix_len, H, nkv, hd, q.device)
     if scratch.buf.get_device() != dev:
@@ -341,8 +344,9 @@ def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
         with ctx:
             return sample_batch(logits, u, temperature, top_k, top_p, min_p, out)
     if out is None:
-        whole = torch.empty((3, n), dtype=_I32, device=logits.device)
-        out = (whole[0], whole[1], whole[2].view(_F32))
+        where = logits.device
+        out = (torch.empty(n, dtype=_I32, device=where), torch.empty(n, dtype=_I32, device=where),
+               torch.empty(n, dtype=_F32, device=where))
     token, kept, prob = out
     check(lib().hyb_sample_batch(logits.data_ptr(), 1 if dtype is _F32 else 0, n, V, ld, *args, _ck("token", token, _I32, rows, dev),
                                  _ck("kept", kept, _I32, rows, dev), _ck("prob", prob, _F32, rows, dev), _here(dev)))

@@ -42,7 +42,10 @@ constexpr int kTileRows = 16;
 constexpr int kWarps = 4;
 constexpr int kSlice = 16;  // keys of one warp step
 
-SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv, int hd) {
+constexpr int kMinSlices = 4;     // of a warp's share: a shorter one is all latency
+constexpr int kCtas = 2 * 148;    // two on every SM of a B200
+
+SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv, int hd, int window) {
     SharedPlan s;
     const int G = n_heads / n_kv;
     max_q = std::min(max_q, T);
@@ -53,38 +56,50 @@ SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len,
     if (req_rows > kTileRows && 4ll * n_req * tiles(req_rows, kTcRows) <= 5ll * tiles(all_rows, kTcRows)) {
         s.tc_per_request = 1;
         s.tc_tiles = tiles(req_rows, kTcRows);
-    } else if (prefix_len > 128 && all_rows > kTileRows) {
-        s.tc_tiles = tiles(all_rows, kTcRows);
-    }
-    if (s.tc_tiles > 0) {
-        const long long units = static_cast<long long>(s.tc_tiles) * n_kv * (s.tc_per_request ? n_req : 1);
-        const long long blocks = (static_cast<long long>(prefix_len) + (s.tc_per_request ? max_own : 0) + 63) / 64;
+        const long long units = static_cast<long long>(s.tc_tiles) * n_kv * n_req;
+        const long long blocks = (static_cast<long long>(prefix_len) + max_own + 63) / 64;
         s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((blocks + 1) / 2, 148 / units)));
-        if (s.tc_per_request) return s;
+        return s;
     }
-    // A single request shares with nobody, and a short prefix costs less to read again than
-    // to treat apart.
-    s.o_prefix = s.tc_tiles == 0 && prefix_len > 0 && (n_req == 1 || prefix_len <= 128);
-    const bool prefix_items = s.tc_tiles == 0 && prefix_len > 0 && !s.o_prefix;
-    const long long keys_o = static_cast<long long>(max_own) + (s.o_prefix ? prefix_len : 0);
-    s.tiles_o = keys_o > 0 ? tiles(req_rows, kTileRows) : 0;
-    s.tiles_p = prefix_items ? tiles(all_rows, kTileRows) : 0;
-    // Parts of about the same length: as many as two CTAs on every SM take at once, of 64 keys
-    // (a shorter part is all latency) to 256 KB of K and V (the SMs finish within one part of each
-    // other). Half of max_own stands for the requests' mean.
-    const long long units_o = static_cast<long long>(s.tiles_o) * n_kv * n_req, units_p = static_cast<long long>(s.tiles_p) * n_kv;
-    const long long work = units_o * (s.o_prefix ? prefix_len + max_own / 2 : max_own / 2) + units_p * prefix_len;
-    const long long part = std::min<long long>(1024, std::max<long long>(64, (work / 296 + 63) / 64 * 64));
-    if (s.tiles_p > 0) s.split_p = static_cast<int>((prefix_len + part - 1) / part);
-    if (s.tiles_o > 0) {
-        s.chunk_o = static_cast<int>(part / kSlice);
-        s.split_o = static_cast<int>(((prefix_len * (s.o_prefix ? 1ll : 0ll) + kSlice - 1) / kSlice + (max_own + kSlice - 1) / kSlice + s.chunk_o - 1) / s.chunk_o);
+    const int tiles_o = tiles(req_rows, kTileRows);
+    const long long units_o = static_cast<long long>(n_req) * tiles_o * n_kv;
+    const long long seen = window > 0 ? std::min(prefix_len, window) : prefix_len;  // of the prefix, by one row at most
+    if (prefix_len > 0) {
+        // The prefix apart, read once for all rows, or again for every request (from L2) in one go with
+        // its own keys? The 16-row kernel gets through some 650 slices of head_dim 256 in a
+        // microsecond then (L2's rate); the 128-row kernel takes about 10 us to start, end and be joined
+        // and 1.2 us a block of head_dim 256 on each SM. A single request shares with nobody.
+        const double again = static_cast<double>(units_o) * ((seen + kSlice - 1) / kSlice) * hd / (256 * 650.);
+        const int tc_tiles = tiles(all_rows, kTcRows);
+        const double apart = 10 + 1.2 * std::max(1., static_cast<double>(tc_tiles) * n_kv * ((seen + 63) / 64) / 148) * hd / 256;
+        if (all_rows <= kTileRows) s.o_prefix = n_req == 1 || prefix_len <= 128;
+        else s.o_prefix = again < apart;
+        if (!s.o_prefix) {
+            if (all_rows <= kTileRows) {
+                s.prefix_unit = 1;
+            } else {
+                s.tc_tiles = tc_tiles;
+                const long long units = static_cast<long long>(tc_tiles) * n_kv;
+                s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((seen + 127) / 128, 148 / units)));
+            }
+        }
     }
+    const long long unit_slices = (max_own + kSlice - 1) / kSlice + (s.o_prefix ? (prefix_len + kSlice - 1) / kSlice : 0);
+    if (unit_slices > 0) s.tiles_o = tiles_o;
+    if (s.tiles_o > 0 && s.tc_tiles == 0 && s.prefix_unit == 0 && unit_slices <= 4 * kMinSlices) {
+        s.one_part = 1;
+        return s;
+    }
+    const long long slices = (s.tiles_o > 0 ? units_o * unit_slices : 0) + static_cast<long long>(s.prefix_unit) * n_kv * ((prefix_len + kSlice - 1) / kSlice);
+    // as many shares of every KV head as fill two CTAs an SM
+    const long long head_slices = slices / n_kv;
+    s.shares = static_cast<int>(std::max<long long>(1, std::min<long long>(kCtas * kWarps / n_kv, head_slices / kMinSlices)));
+    if (slices == 0) s.shares = 0;
     return s;
 }
 
-// The keys of one segment (prefix or own) for a tile of rows: those in [lo, hi) are seen by some
-// row, its slices start at key `first`.
+// The keys of one segment (prefix or own) for some rows: those in [lo, hi) are seen by one of
+// them (for rows at neighbouring positions), the slices start at key `first`.
 struct Keys {
     const int* table;
     int base, lo, hi, first, slices;
@@ -97,10 +112,28 @@ __device__ __forceinline__ Keys keys_of(const int* table, int base, int len, int
     k.lo = 0;
     if (window > 0) k.lo = static_cast<int>(min(static_cast<long long>(k.hi), max(0ll, static_cast<long long>(pmin) - window + 1 - base)));
     k.first = k.lo & ~(kSlice - 1);
-    // without a window the slices depend on the length alone, so that their pages can be looked
-    // up before the rows' positions are known
+    // without a window the slices depend on the length alone, so that shares can be cut and pages
+    // looked up before the rows' positions are known
     k.slices = window > 0 ? (k.hi > k.lo ? (k.hi - k.first + kSlice - 1) / kSlice : 0) : (len + kSlice - 1) / kSlice;
     return k;
+}
+
+// The rows of request `req` (-1: all), its own keys within the bounds, and whether it breaks them.
+struct Request {
+    int t0, n_tok, own;
+    bool broken;
+};
+__device__ __forceinline__ Request request_of(const SharedAttnParams& p, int req) {
+    Request r = {0, p.T, 0, false};
+    if (req >= 0) {
+        const int a = p.row_start[req], b = p.row_start[req + 1], len = p.own_lens[req];
+        const long long most = min(static_cast<long long>(p.max_own), static_cast<long long>(p.max_blocks) * p.page_size);
+        r.t0 = min(max(a, 0), p.T);
+        r.n_tok = max(0, min(min(b, p.T) - r.t0, p.max_q));
+        r.own = static_cast<int>(min(static_cast<long long>(max(0, len)), most));
+        r.broken = len > most;
+    }
+    return r;
 }
 
 template <int HD>
@@ -112,21 +145,27 @@ struct SmallPlan {
     static constexpr int kRing = kWarps * kStages * kHalf;
     static constexpr int kMerge = kWarps * kTileRows * HD * 4;
     static constexpr int kBars = kRing > kMerge ? kRing : kMerge;
-    static constexpr int kSmem = kBars + kWarps * kStages * 8 + 1024;  // + alignment slack
+    static constexpr int kStart = kBars + kWarps * kStages * 8;  // per request: first slice, slices of a unit
+    static constexpr int kSmem = kStart + 2 * kMaxSharedRequests * 4 + 1024;  // + alignment slack
 };
 
-// One CTA: up to 16 rows (row m of a tile = token m / G, head m % G of the KV head's group)
-// against one part of the prefix, or of one request's keys. Each warp takes every fourth
-// 16-key slice of the part on its own: tensor-map copies into its own ring, QK^T and PV on
-// mma.sync m16n8k16, online softmax; the four warps' results are joined at the end. V rows
-// of keys that no row of the tile sees are cleared before the product (0 * NaN). Rows
-// share every byte of K and V that is loaded, so up to 16 rows cost the same traffic as one:
-// HBM bound, if the eight warps of an SM get through a slice in 1.5 us at head_dim 128; so
-// copies are issued for a whole slice at once (per-lane 16-byte copies took half of 660
-// instructions a slice), and masks and rescaling sit behind warp-uniform branches.
-// The chain in front of the first copy is three loads deep: lengths, row starts and pages;
-// positions; keys.
-template <int HD>
+// Up to 16 rows (row m of a tile = token m / G, head m % G of the KV head's group) against 16-key
+// slices, on mma.sync m16n8k16 with an online softmax, each warp on its own: tensor-map copies
+// into its own ring, V rows of keys that no row of the request sees cleared before the product
+// (0 * NaN). Rows share every byte of K and V that is loaded, so up to 16 rows cost the same
+// traffic as one: HBM bound, if the eight warps of an SM get through a slice in 1.5 us at
+// head_dim 128; so copies are issued for a whole slice at once (per-lane 16-byte copies took half
+// of 660 instructions a slice), and masks and rescaling sit behind warp-uniform branches.
+//
+// A unit is a tile of rows with the keys it has to see: the batch's rows with the prefix, or one
+// request's with its own keys (o_prefix: the prefix in front). All units' slices in a row are cut
+// into equal shares, whatever the requests' lengths (each CTA adds the lengths up itself); a warp
+// takes a share for one KV head, writes what it has for a unit (a piece) and goes on with the next.
+// Neighbouring warps take the same share for neighbouring heads, whose keys are neighbours in
+// memory: with the heads one after the other in the row of slices the same kernel reached half
+// the bandwidth. ONE: short units, a CTA takes a whole one, joins its four warps and writes
+// the output itself.
+template <int HD, bool ONE>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     shared_attn_small_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                              const SharedAttnParams p, const SharedPlan pl, SharedParts parts, int after_tc) {
@@ -145,57 +184,139 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     mbar_init_fence();
     __syncwarp();
 
-    // ---- which part
-    int id = blockIdx.x;
-    const int n_prefix = pl.tiles_p * p.n_kv * pl.split_p;
-    const bool prefix = id < n_prefix;
-    int split, hk, tile, req = 0;
-    if (prefix) {
-        split = id % pl.split_p;
-        id /= pl.split_p;
-        hk = id % p.n_kv;
-        tile = id / p.n_kv;
+    // this warp's share [r0, r1) of the slices, for head my_hk
+    unsigned* s_start = reinterpret_cast<unsigned*>(sm + SP::kStart);
+    int* s_slices = reinterpret_cast<int*>(s_start + kMaxSharedRequests);
+    unsigned r0 = 0, r1 = 0, prefix_slices = 0;
+    const int my_warp = blockIdx.x * kWarps + warp, my_share = my_warp / p.n_kv, my_hk = my_warp % p.n_kv;
+    if constexpr (!ONE) {
+        // positions matter for the number of slices only where a window cuts the keys
+        auto span = [&](const Request& r, int& lo, int& hi) {
+            lo = INT_MAX;
+            hi = -1;
+            for (int t = 0; p.window > 0 && t < r.n_tok; ++t) {
+                const int pos = p.row_pos[r.t0 + t];
+                if (pos >= 0) {
+                    lo = min(lo, pos);
+                    hi = max(hi, pos);
+                }
+            }
+        };
+        int lo, hi;
+        if (pl.prefix_unit) {
+            span(request_of(p, -1), lo, hi);
+            prefix_slices = keys_of(nullptr, 0, p.prefix_len, lo, hi, p.window).slices;
+        }
+        const int per = (p.n_req + kWarps * 32 - 1) / (kWarps * 32);
+        const int b0 = min(p.n_req, static_cast<int>(threadIdx.x) * per), b1 = min(p.n_req, b0 + per);
+        unsigned sum = 0;
+        for (int b = b0; b < b1 && pl.tiles_o > 0; ++b) {
+            const Request r = request_of(p, b);
+            span(r, lo, hi);
+            const int n = keys_of(nullptr, p.prefix_len, r.own, lo, hi, p.window).slices +
+                          (pl.o_prefix ? keys_of(nullptr, 0, p.prefix_len, lo, hi, p.window).slices : 0);
+            s_slices[b] = n;
+            s_start[b] = sum;
+            sum += static_cast<unsigned>(n) * ((r.n_tok * G + kTileRows - 1) / kTileRows);
+        }
+        unsigned before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
+        }
+        if (lane == 31) s_row[warp] = static_cast<int>(before);
+        __syncthreads();
+        before -= sum;
+        unsigned total = prefix_slices;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_row[w];
+            total += s_row[w];
+        }
+        for (int b = b0; b < b1; ++b) s_start[b] += prefix_slices + before;
+        __syncthreads();
+        if (pl.tiles_o == 0) {
+            for (int b = b0; b < b1; ++b) s_slices[b] = 0;
+            __syncthreads();
+        }
+        const unsigned shares = min(static_cast<unsigned>(pl.shares), max(1u, total / kMinSlices));
+        if (my_share < static_cast<int>(shares)) {
+            r0 = static_cast<unsigned>(static_cast<uint64_t>(my_share) * total / shares);
+            r1 = static_cast<unsigned>(static_cast<uint64_t>(my_share + 1) * total / shares);
+        }
+        // which shares have a piece of a unit: for the merge, every unit by one CTA
+        auto pieces = [&](unsigned a, int n) {
+            if (total == 0 || n == 0) return make_int2(0, 0);
+            const unsigned w0 = static_cast<unsigned>((static_cast<uint64_t>(a + 1) * shares - 1) / total);
+            const unsigned w1 = static_cast<unsigned>((static_cast<uint64_t>(a + n) * shares - 1) / total);
+            return make_int2(static_cast<int>(w0), static_cast<int>(w1 - w0 + 1));
+        };
+        if (blockIdx.x == 0 && threadIdx.x == 0 && pl.prefix_unit) parts.unit[0] = pieces(0, prefix_slices);
+        for (int i = blockIdx.x * kWarps * 32 + threadIdx.x; i < p.n_req * pl.tiles_o; i += gridDim.x * kWarps * 32) {
+            const int b = i / pl.tiles_o;
+            parts.unit[pl.prefix_unit + i] = pieces(s_start[b] + (i - b * pl.tiles_o) * s_slices[b], s_slices[b]);
+        }
+    }
+
+    int slot = 0, phase = 0;  // the ring's next stage
+    bool ok = true;
+#pragma unroll 1
+    for (bool more = true; more;) {
+    // ---- which unit, and which of its slices: i-th one s0 + i * stride
+    int req, tile, hk, s0, mine, unit;
+    constexpr int stride = ONE ? kWarps : 1;
+    if constexpr (ONE) {
+        hk = blockIdx.x % p.n_kv;
+        unit = blockIdx.x / p.n_kv;
+        tile = unit % pl.tiles_o;
+        req = unit / pl.tiles_o;
+        s0 = warp;
+        mine = 0;
+        more = false;
     } else {
-        id -= n_prefix;
-        hk = id % p.n_kv;
-        id /= p.n_kv;
-        split = id % pl.split_o;
-        id /= pl.split_o;
-        tile = id % pl.tiles_o;
-        req = id / pl.tiles_o;
+        if (r0 >= r1) break;
+        int n;
+        hk = my_hk;
+        if (r0 < prefix_slices) {
+            unit = 0;
+            tile = 0;
+            req = -1;
+            n = prefix_slices;
+            s0 = r0;
+        } else {
+            int lo = 0, hi = p.n_req;  // the last request that starts at or before r0 (it has slices)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (s_start[mid] <= r0) lo = mid;
+                else hi = mid;
+            }
+            req = lo;
+            n = s_slices[req];
+            const int rel = r0 - s_start[req];
+            tile = rel / n;
+            unit = pl.prefix_unit + req * pl.tiles_o + tile;
+            s0 = rel - tile * n;
+        }
+        mine = min(static_cast<int>(r1 - r0), n - s0);
+        r0 += mine;
     }
-    // ---- lengths, row starts
-    int t0 = 0, n_tok = p.T, own = 0;
-    const long long most = min(static_cast<long long>(p.max_own), static_cast<long long>(p.max_blocks) * p.page_size);
-    bool broken = false;
-    if (!prefix) {
-        const int a = p.row_start[req], b = p.row_start[req + 1], len = p.own_lens[req];
-        t0 = min(max(a, 0), p.T);
-        n_tok = min(min(b, p.T) - t0, p.max_q);
-        own = static_cast<int>(min(static_cast<long long>(max(0, len)), most));
-        broken = len > most;
-    }
-    const int len_p = prefix || pl.o_prefix ? p.prefix_len : 0;
-    const int per = prefix ? 0 : pl.chunk_o;
-    const int* own_table = p.table + static_cast<size_t>(req) * p.max_blocks;
+    const Request rq = request_of(p, req);
+    const int t0 = rq.t0, len_p = req < 0 || pl.o_prefix ? p.prefix_len : 0;
+    const int* own_table = p.table + static_cast<size_t>(max(req, 0)) * p.max_blocks;
     // ---- the pages of this warp's first 32 slices, one a lane, while no window moves the slices
     int pages = 0;
     const int slices_p = (len_p + kSlice - 1) / kSlice;
-    // a prefix item splits the prefix evenly, in steps of 64 keys
-    const int per_p = prefix ? (((p.prefix_len + pl.split_p - 1) / pl.split_p + 63) & ~63) / kSlice : 0;
     if (p.window == 0) {
-        const int s = split * (prefix ? per_p : per) + warp + lane * kWarps;
+        const int s = s0 + lane * stride;
         if (s < slices_p) pages = p.prefix_table[s * kSlice / p.page_size];
-        else if (!prefix && s - slices_p < (own + kSlice - 1) / kSlice) pages = own_table[(s - slices_p) * kSlice / p.page_size];
+        else if (s - slices_p < (rq.own + kSlice - 1) / kSlice) pages = own_table[(s - slices_p) * kSlice / p.page_size];
     }
-    if (parts.direct && tile == pl.tiles_o - 1 && split == 0) shared_fill_unserved(p, req, hk, t0, kWarps * 32);
+    if (ONE && tile == pl.tiles_o - 1) shared_fill_unserved(p, req, hk, t0, kWarps * 32);
     // ---- rows m0 .. m0 + rows of the (token, head) pairs from token t0 on
     const int m0 = tile * kTileRows;
-    const int rows = static_cast<int>(max(0ll, min(static_cast<long long>(kTileRows), static_cast<long long>(n_tok) * G - m0)));
-    if (rows <= 0) {
-        if (after_tc) pdl_wait();
-        return;
-    }
+    const int rows = static_cast<int>(max(0ll, min(static_cast<long long>(kTileRows), static_cast<long long>(rq.n_tok) * G - m0)));
+    if (ONE && rows <= 0) return;
     // lane m (and m + 16): row m's position and place
     const int mm = m0 + min(lane & 15, rows - 1), tok = mm / G;
     const int my_pos = (lane & 15) < rows ? p.row_pos[t0 + tok] : -1;
@@ -213,18 +334,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             qf[k][3] = *reinterpret_cast<const uint32_t*>(qb + 16 * k + 8 + c2);
         }
     }
-    if (warp == 0 && lane < kTileRows) s_row[lane] = my_row | (my_pos < 0 ? 0x80000000 : 0);
-    const int pmin = __reduce_min_sync(0xffffffffu, my_pos < 0 ? INT_MAX : my_pos);
-    const int pmax = __reduce_max_sync(0xffffffffu, my_pos);
+    if (ONE && warp == 0 && lane < kTileRows) s_row[lane] = my_row | (my_pos < 0 ? 0x80000000 : 0);
+    // the span of the tile's positions; of the request's where a window cuts the keys by it
+    int pmin = my_pos < 0 ? INT_MAX : my_pos, pmax = my_pos;
+    if (!ONE && p.window > 0)
+        for (int t = lane; t < rq.n_tok; t += 32) {
+            const int pos = p.row_pos[t0 + t];
+            if (pos >= 0) pmin = min(pmin, pos);
+            pmax = max(pmax, pos);
+        }
+    pmin = __reduce_min_sync(0xffffffffu, pmin);
+    pmax = __reduce_max_sync(0xffffffffu, pmax);
     const int posA = __shfl_sync(0xffffffffu, my_pos, g), posB = __shfl_sync(0xffffffffu, my_pos, g + 8);
-    // ---- its keys: slices [s0, s1) of the prefix's, then the request's own
+    // ---- its keys: the prefix's slices, then the request's own
     const Keys ka = keys_of(p.prefix_table, 0, len_p, pmin, pmax, p.window);
-    const Keys kb = keys_of(own_table, p.prefix_len, own, pmin, pmax, p.window);
-    const int total = ka.slices + kb.slices;
-    const int step = !prefix ? per : (p.window == 0 ? per_p : (ka.slices + pl.split_p - 1) / pl.split_p);
-    const int s0 = static_cast<int>(min(static_cast<long long>(total), static_cast<long long>(split) * step));
-    const int s1 = min(total, s0 + step);
-    const int mine = s1 - s0 > warp ? (s1 - s0 - warp + kWarps - 1) / kWarps : 0;
+    const Keys kb = keys_of(own_table, p.prefix_len, rq.own, pmin, pmax, p.window);
+    if (ONE) mine = ka.slices + kb.slices > warp ? (ka.slices + kb.slices - warp + kWarps - 1) / kWarps : 0;
 
     float o[HD / 8][4];
 #pragma unroll
@@ -234,10 +359,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
     bool bad = false;
 
-    bool ok = true;
     const int page_shift = __ffs(p.page_size) - 1, in_page = p.page_size - 1;
     auto load_pages = [&](int from) {  // of this warp's slices from .. from + 31, as first slots
-        const int i = from + lane, s = s0 + warp + i * kWarps;
+        const int i = from + lane, s = s0 + i * stride;
         const bool a = s < ka.slices;
         const int key = a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
         if ((from > 0 || p.window > 0) && i < mine) pages = (a ? ka.table : kb.table)[key >> page_shift];
@@ -246,7 +370,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         // slices without a visible key, and bad pages: a box past the pool, which reads as zeros
         pages = i < mine && there && key < (a ? ka.hi : kb.hi) ? (pages << page_shift) + (key & in_page) : p.n_pages << page_shift;
     };
-    int f_slot = 0;
+    int f_slot = slot;
     auto fetch = [&](int j) {  // K (even) or V (odd) of this warp's slice j / 2
         const int i = j >> 1;
         if (i < mine) {
@@ -275,10 +399,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             v_off[c] = vk * 128 + (((2 * c + vh) ^ (vk & 7)) << 4);
         }
     }
-    int slot = 0, phase = 0;
     for (int i = 0; i < mine; ++i) {
         fetch(2 * i + ST - 1);
-        const int s = s0 + warp + i * kWarps;
+        const int s = s0 + i * stride;
         const bool in_a = s < ka.slices;
         const int key0 = in_a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
         const int lo = in_a ? ka.lo : kb.lo, hi = in_a ? ka.hi : kb.hi, base = in_a ? 0 : p.prefix_len;
@@ -378,134 +501,173 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
         __syncwarp();  // and the V stage
     }
-    if (!ok) {
-        // a wait gave up: give copies that may still be in flight the same time again
-        const uint64_t from = shared_now_ns();
-        while (shared_now_ns() - from < 500000000ull) __nanosleep(1000);
-    }
 #pragma unroll
     for (int w = 1; w <= 2; w <<= 1) {
         lA += __shfl_xor_sync(0xffffffffu, lA, w);
         lB += __shfl_xor_sync(0xffffffffu, lB, w);
     }
     // a page outside the pool: the rows of the tile come out as NaN, not as a silent subset
-    if (__any_sync(0xffffffffu, bad) || (broken && parts.direct)) {
+    if (__any_sync(0xffffffffu, bad) || (ONE && rq.broken)) {
         lA = lB = __int_as_float(0x7fffffff);
         mA = mB = 0.f;
     }
-    if ((lane & 3) == 0) {
-        s_m[warp][g] = mA;
-        s_m[warp][g + 8] = mB;
-        s_l[warp][g] = lA;
-        s_l[warp][g + 8] = lB;
-    }
-    __syncthreads();  // statistics written; every warp is done with its ring
-    float* so = reinterpret_cast<float*>(sm) + warp * kTileRows * HD;
+    if constexpr (!ONE) {
+        const size_t place = (static_cast<size_t>(my_share + unit) * p.n_kv + hk) * kTileRows;
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) {
-        *reinterpret_cast<float2*>(so + g * HD + 8 * d + c2) = make_float2(o[d][0], o[d][1]);
-        *reinterpret_cast<float2*>(so + (g + 8) * HD + 8 * d + c2) = make_float2(o[d][2], o[d][3]);
-    }
-    __syncthreads();
-    const int at = pl.tc_splits + (prefix ? split : pl.split_p + split);
-    for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += kWarps * 32) {
-        const int m = idx / (HD / 4), d = 4 * (idx % (HD / 4));
-        float M = -INFINITY;
+        for (int half = 0; half < 2; ++half) {
+            const int m = g + 8 * half;
+            const float l = half ? lB : lA;
+            if (m >= rows) continue;
+            if ((lane & 3) == 0) parts.pml[place + m] = make_float2(half ? mB : mA, l);
+            if (l == 0.f) continue;
+            float* dst = parts.po + (place + m) * HD + c2;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][m]);
-        const float z = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = shared_ex2(s_m[w][m] - z);
-            const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm) + (w * kTileRows + m) * HD + d);
-            L += f * s_l[w][m];
-            acc.x += f * x.x;
-            acc.y += f * x.y;
-            acc.z += f * x.z;
-            acc.w += f * x.w;
+            for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(o[d][2 * half], o[d][2 * half + 1]);
         }
-        const size_t row = static_cast<size_t>(s_row[m] & 0x7fffffff);
-        if (!parts.direct) {
-            if (L != 0.f) *reinterpret_cast<float4*>(parts.o + (row * parts.n + at) * HD + d) = acc;
-            if (d == 0) parts.ml[row * parts.n + at] = make_float2(M, L);
-        } else if (s_row[m] >= 0) {  // the only part of its rows: the output itself
+    } else {
+        if ((lane & 3) == 0) {
+            s_m[warp][g] = mA;
+            s_m[warp][g + 8] = mB;
+            s_l[warp][g] = lA;
+            s_l[warp][g + 8] = lB;
+        }
+        __syncthreads();  // statistics written; every warp is done with its ring
+        float* so = reinterpret_cast<float*>(sm) + warp * kTileRows * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) {
+            *reinterpret_cast<float2*>(so + g * HD + 8 * d + c2) = make_float2(o[d][0], o[d][1]);
+            *reinterpret_cast<float2*>(so + (g + 8) * HD + 8 * d + c2) = make_float2(o[d][2], o[d][3]);
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < rows * (HD / 4); idx += kWarps * 32) {
+            const int m = idx / (HD / 4), d = 4 * (idx % (HD / 4));
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][m]);
+            const float z = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = shared_ex2(s_m[w][m] - z);
+                const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm) + (w * kTileRows + m) * HD + d);
+                L += f * s_l[w][m];
+                acc.x += f * x.x;
+                acc.y += f * x.y;
+                acc.z += f * x.z;
+                acc.w += f * x.w;
+            }
+            if (s_row[m] < 0) continue;
             const float inv = L > 0.f ? 1.0f / L : L;
-            *reinterpret_cast<uint2*>(p.out + row * HD + d) =
+            *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(s_row[m]) * HD + d) =
                 make_uint2(pack_bf2(f2bf(acc.x * inv), f2bf(acc.y * inv)), pack_bf2(f2bf(acc.z * inv), f2bf(acc.w * inv)));
         }
+    }
+    }
+    if (!ok) {
+        // a wait gave up: give copies that may still be in flight the same time again
+        const uint64_t from = shared_now_ns();
+        while (shared_now_ns() - from < 500000000ull) __nanosleep(1000);
     }
     // this grid may start under the 128-row kernel's last CTAs; it ends after them, so that the
     // merge, which waits for this grid, waits for both
     if (after_tc) pdl_wait();
 }
 
-// W warps per (row, head) join its parts, each every W-th. Rows before row_start[0] or from
+// W warps per (row, head) join its parts, each every W-th: those of the 128-row kernel, the pieces of
+// its prefix unit, the pieces of its request's unit. Rows before row_start[0] or from
 // row_start[n_req] on belong to no request and are left as they were; a row whose request
 // breaks the bounds the caller gave (more rows than max_q, more keys than max_own or its
 // table) has parts that were not computed and becomes NaN.
 template <int HD>
-__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParams p, SharedParts parts, int W) {
+__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParams p, const SharedPlan pl, SharedParts parts, int W) {
     constexpr int PER = HD / 32;
     __shared__ float s_o[8][HD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % W;
-    const long long unit = (static_cast<long long>(blockIdx.x) * 8 + warp) / W;
-    const int t = static_cast<int>(min(unit / p.n_heads, static_cast<long long>(p.T)));
+    const long long row = (static_cast<long long>(blockIdx.x) * 8 + warp) / W;
+    const int t = static_cast<int>(min(row / p.n_heads, static_cast<long long>(p.T)));
     bool live = t < p.T, broken = false;
-    if (live) {
-        live = t >= p.row_start[0] && t < p.row_start[p.n_req] && p.row_pos[t] >= 0;
+    // the last request that starts at or before t: 32 starts a step, by the whole warp
+    int req = 0, first = 0;
+    {
+        const int step = (p.n_req + 31) / 32, end = p.row_start[p.n_req], pos = live ? p.row_pos[t] : -1;
+        int v = lane * step < p.n_req ? p.row_start[lane * step] : INT_MAX;
+        const int begin = __shfl_sync(0xffffffffu, v, 0);
+        req = max(0, __popc(__ballot_sync(0xffffffffu, v <= t)) - 1) * step;
+        first = __shfl_sync(0xffffffffu, v, req / step);
+        if (step > 1) {
+            v = lane < step && req + lane < p.n_req ? p.row_start[req + lane] : INT_MAX;
+            const int more = max(0, __popc(__ballot_sync(0xffffffffu, v <= t)) - 1);
+            req += more;
+            first = __shfl_sync(0xffffffffu, v, more);
+        }
+        live = live && t >= begin && t < end && pos >= 0;
         if (live) {
-            int lo = 0, hi = p.n_req;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (p.row_start[mid] <= t) lo = mid;
-                else hi = mid;
-            }
-            const int own = p.own_lens[lo];
-            broken = t - p.row_start[lo] >= p.max_q || own > p.max_own ||
-                     own > static_cast<long long>(p.max_blocks) * p.page_size;
+            const int own = p.own_lens[req];
+            broken = t - first >= p.max_q || own > p.max_own || own > static_cast<long long>(p.max_blocks) * p.page_size;
         }
     }
     pdl_wait();
     float L = 0.f, acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    if (live) {
-        const float2* ml = parts.ml + static_cast<size_t>(unit) * parts.n;
-        const float* src = parts.o + static_cast<size_t>(unit) * parts.n * HD + lane * PER;
-        float M = -INFINITY;
-        for (int s = lane; s < parts.n; s += 32) M = fmaxf(M, ml[s].x);
+    if (live && !broken) {
+        const int G = p.n_heads / p.n_kv, h = static_cast<int>(row % p.n_heads), hk = h / G, g = h - hk * G;
+        // its pieces: n0 of the prefix's unit from place a0 on, at row m0; n1 of its request's, at row m1
+        long long a0 = 0, a1 = 0;
+        int n0 = 0, n1 = 0, m0 = 0, m1 = 0;
+        if (pl.prefix_unit) {
+            const int2 u = parts.unit[0];  // one tile
+            a0 = u.x;
+            n0 = u.y;
+            m0 = t * G + g;
+        }
+        if (pl.tiles_o > 0) {
+            const int m = (t - first) * G + g, unit = pl.prefix_unit + req * pl.tiles_o + m / kTileRows;
+            const int2 u = parts.unit[unit];
+            a1 = u.x + unit;
+            n1 = u.y;
+            m1 = m % kTileRows;
+        }
+        const int n = parts.n + n0 + n1;
+        auto place = [&](int s) {  // of part s - parts.n, in rows
+            s -= parts.n;
+            return (((s < n0 ? a0 + s : a1 + s - n0) * p.n_kv + hk) * kTileRows) + (s < n0 ? m0 : m1);
+        };
+        auto stat = [&](int s) { return s < parts.n ? parts.ml[row * parts.n + s] : parts.pml[place(s)]; };
+        const float2 v0 = lane < n ? stat(lane) : make_float2(-INFINITY, 0.f);  // mostly all there is
+        float M = v0.x;
+        for (int s = 32 + lane; s < n; s += 32) M = fmaxf(M, stat(s).x);
         M = warp_max(M);
         const float z = M == -INFINITY ? 0.f : M;
-        for (int s0 = 0; s0 < parts.n; s0 += 32) {
-            float f = 0.f, fl = 0.f;
-            if (s0 + lane < parts.n) {
-                const float2 v = ml[s0 + lane];
-                f = v.y == 0.f ? 0.f : shared_ex2(v.x - z);  // l = 0: no key of the part is seen, no output written
-                fl = f * v.y;
-            }
-            L += warp_sum(fl);
-            const int n = min(32, parts.n - s0);
-#pragma unroll 4
-            for (int s = sub; s < n; s += W) {
-                const float fs = __shfl_sync(0xffffffffu, f, s);
-                if (fs == 0.f) continue;
-                const float* at = src + static_cast<size_t>(s0 + s) * HD;
-                if constexpr (PER == 2) {
-                    const float2 x = *reinterpret_cast<const float2*>(at);
-                    acc[0] += fs * x.x;
-                    acc[1] += fs * x.y;
-                } else {
+        for (int s0 = 0; s0 < n; s0 += 32) {
+            const float2 v = s0 == 0 ? v0 : (s0 + lane < n ? stat(s0 + lane) : make_float2(-INFINITY, 0.f));
+            const float f = v.y == 0.f ? 0.f : shared_ex2(v.x - z);  // l = 0: no key of the part is seen, no output written
+            L += warp_sum(f * v.y);
+            const int e = min(32, n - s0);
+            constexpr int U = 4;  // parts whose loads are in flight together
+            for (int s1 = sub; s1 < e; s1 += U * W) {
+                float x[U][PER], fs[U];
 #pragma unroll
-                    for (int i = 0; i < PER; i += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(at + i);
-                        acc[i] += fs * x.x;
-                        acc[i + 1] += fs * x.y;
-                        acc[i + 2] += fs * x.z;
-                        acc[i + 3] += fs * x.w;
+                for (int q = 0; q < U; ++q) {
+                    const int s = s1 + q * W;
+                    fs[q] = __shfl_sync(0xffffffffu, f, s & 31);
+                    if (s >= e) fs[q] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) x[q][i] = 0.f;
+                    if (fs[q] == 0.f) continue;
+                    const float* at = (s0 + s < parts.n ? parts.o + (row * parts.n + s0 + s) * HD : parts.po + place(s0 + s) * HD) + lane * PER;
+                    if constexpr (PER == 2) {
+                        *reinterpret_cast<float2*>(x[q]) = *reinterpret_cast<const float2*>(at);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4*>(x[q] + i) = *reinterpret_cast<const float4*>(at + i);
                     }
                 }
+#pragma unroll
+                for (int q = 0; q < U; ++q)
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) acc[i] += fs[q] * x[q][i];
             }
         }
     }
@@ -521,51 +683,75 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParam
     if (!live) return;
     float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // no key seen: zeros; NaN stays
     if (broken) inv = __int_as_float(0x7fffffff);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(unit) * HD + lane * PER);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * HD + lane * PER);
 #pragma unroll
     for (int i = 0; i < PER / 2; ++i) dst[i] = pack_bf2(f2bf(acc[2 * i] * inv), f2bf(acc[2 * i + 1] * inv));
 }
 
+// Where the parts lie in the scratch.
+struct Layout {
+    long long rows, units, places;
+    size_t o, ml, po, pml, unit, bytes;
+    Layout(const SharedPlan& s, int T, int n_req, int n_heads, int n_kv, int hd) {
+        rows = s.direct() ? 0 : static_cast<long long>(T) * n_heads * s.tc_splits;
+        units = s.direct() ? 0 : s.prefix_unit + static_cast<long long>(n_req) * s.tiles_o;
+        places = s.shares > 0 && !s.direct() ? (units + s.shares) * n_kv : 0;
+        o = 0;
+        ml = o + rows * hd * sizeof(float);
+        po = (ml + rows * sizeof(float2) + 255) & ~static_cast<size_t>(255);
+        pml = po + places * kTileRows * hd * sizeof(float);
+        unit = pml + places * kTileRows * sizeof(float2);
+        bytes = unit + units * sizeof(int2);
+    }
+};
+
 template <int HD>
 void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream) {
     using SP = SmallPlan<HD>;
-    const long long n_prefix = static_cast<long long>(pl.tiles_p) * p.n_kv * pl.split_p;
-    const long long n_req = static_cast<long long>(pl.tiles_o) * p.n_kv * pl.split_o * p.n_req;
     const long long warps = static_cast<long long>(p.T) * p.n_heads;
-    if (n_prefix + n_req > INT_MAX || warps > INT_MAX - 8) throw ArgError("sdpa_shared_prefix: too many parts");
     if (pl.tc_splits > 0) launch_shared_attn_tc(p, pl, parts, stream);
-    if (n_prefix + n_req > 0) {
-        allow_smem(reinterpret_cast<const void*>(shared_attn_small_kernel<HD>), SP::kSmem);
+    if (pl.one_part || pl.shares > 0) {
+        const long long ctas = pl.one_part ? static_cast<long long>(p.n_req) * pl.tiles_o * p.n_kv
+                                           : (static_cast<long long>(pl.shares) * p.n_kv + kWarps - 1) / kWarps;
+        if (ctas > INT_MAX / kTileRows) throw ArgError("sdpa_shared_prefix: too many rows");
         CUtensorMap tk, tv;
         shared_pool_maps(p, kSlice, &tk, &tv);
-        shared_launch(shared_attn_small_kernel<HD>, static_cast<unsigned>(n_prefix + n_req), kWarps * 32, SP::kSmem, stream,
+        auto kern = pl.one_part ? shared_attn_small_kernel<HD, true> : shared_attn_small_kernel<HD, false>;
+        allow_smem(reinterpret_cast<const void*>(kern), SP::kSmem);
+        shared_launch(kern, static_cast<unsigned>(ctas), kWarps * 32, SP::kSmem, stream,
                       pl.tc_splits > 0, tk, tv, p, pl, parts, pl.tc_splits > 0 ? 1 : 0);
     }
     if (parts.direct) return;  // the only part wrote the output
-    // one warp joins a few parts as fast as several: the loads of four are in flight at once
-    const int W = parts.n >= 16 ? 8 : (parts.n >= 8 ? 4 : (parts.n >= 4 ? 2 : 1));
-    shared_launch(shared_merge_kernel<HD>, static_cast<unsigned>((warps * W + 7) / 8), 256, 0, stream, parts.n > 0, p, parts, W);
+    // several warps a row while all of them run at once
+    const int W = warps <= 592 ? 8 : (warps <= 1184 ? 4 : (warps <= 2368 ? 2 : 1));
+    shared_launch(shared_merge_kernel<HD>, static_cast<unsigned>((warps * W + 7) / 8), 256, 0, stream,
+                  pl.tc_splits > 0 || pl.shares > 0, p, pl, parts, W);
 }
 
 }  // namespace
 
 size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
                                  int hd) {
-    const SharedPlan s = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd);
-    const size_t units = s.direct() ? 0 : static_cast<size_t>(T) * n_heads * s.splits();
-    return units * hd * sizeof(float) + units * sizeof(float2) + 512;
+    // For any window: the prefix apart takes most without one (the most parts), together with the
+    // requests' keys the same with any, and the shorter the window the sooner they go together.
+    const SharedPlan none = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd, 0);
+    const SharedPlan least = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd, 1);
+    return std::max(Layout(none, T, n_req, n_heads, n_kv, hd).bytes, Layout(least, T, n_req, n_heads, n_kv, hd).bytes) + 512;
 }
 
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
-    const SharedPlan pl = plan_shared(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd);
-    const size_t units = static_cast<size_t>(p.T) * p.n_heads * pl.splits();
-    if (p.scratch_bytes < shared_attn_scratch_bytes(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd))
-        throw ArgError("sdpa_shared_prefix: scratch too small");
+    const SharedPlan pl = plan_shared(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd, p.window);
+    const Layout at(pl, p.T, p.n_req, p.n_heads, p.n_kv, p.hd);
+    if (p.scratch_bytes < at.bytes + 512) throw ArgError("sdpa_shared_prefix: scratch too small");
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p.scratch) + 255) & ~static_cast<uintptr_t>(255));
     SharedParts parts;
-    parts.o = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(p.scratch) + 255) & ~static_cast<uintptr_t>(255));
-    parts.ml = reinterpret_cast<float2*>(parts.o + units * p.hd);
-    parts.n = pl.splits();
+    parts.o = reinterpret_cast<float*>(base + at.o);
+    parts.ml = reinterpret_cast<float2*>(base + at.ml);
+    parts.n = pl.tc_splits;
     parts.direct = pl.direct();
+    parts.po = reinterpret_cast<float*>(base + at.po);
+    parts.pml = reinterpret_cast<float2*>(base + at.pml);
+    parts.unit = reinterpret_cast<int2*>(base + at.unit);
     switch (p.hd) {
         case 64: launch_shared_t<64>(p, pl, parts, stream); break;
         case 128: launch_shared_t<128>(p, pl, parts, stream); break;

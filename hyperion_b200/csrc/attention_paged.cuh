@@ -69,28 +69,34 @@ __device__ __forceinline__ void shared_tma_load_if(uint32_t dst, const void* map
         : "memory");
 }
 // How a call's rows and keys are split; the same on the host for the scratch size and the
-// grids, and on the device. Parts of a row, in this order: those of the 128-row kernel, the
-// prefix's and the request's own ones of the 16-row kernel.
+// grids, and on the device.
 struct SharedPlan {
     int tc_splits = 0;       // parts of the 128-row kernel (0: not launched)
     int tc_tiles = 0;        // 128-row tiles over all rows, or of one request
     int tc_per_request = 0;  // tiles hold one request's rows and cover prefix and own keys
-    int tiles_p = 0, split_p = 0;  // 16-row tiles over all rows; parts of the prefix
-    int tiles_o = 0, split_o = 0;  // 16-row tiles of one request; parts of its keys
-    int chunk_o = 0;               // 16-key slices of one part
-    int o_prefix = 0;              // a request's 16-row tiles cover the prefix too
-    __host__ __device__ int splits() const { return tc_splits + split_p + split_o; }
-    // one part, of tiles that hold the rows of one request: it writes the output itself
-    bool direct() const { return splits() == 1 && (tc_per_request != 0 || split_o == 1); }
+    int prefix_unit = 0;     // 16-row kernel: one tile of all rows against the prefix
+    int tiles_o = 0;         // 16-row tiles of one request (0: not launched)
+    int o_prefix = 0;        // they cover the prefix too
+    int one_part = 0;        // a CTA takes a whole unit and writes the output
+    int shares = 0;          // otherwise: shares of every KV head's slices, a warp each
+    // nothing has to be joined
+    __host__ __device__ bool direct() const { return one_part != 0 || (tc_per_request != 0 && tc_splits == 1); }
 };
 
-// Scratch: fp32 partial outputs [T][n_heads][n][hd], then (m, l) pairs [T][n_heads][n]; m in
-// powers of two. A part with l = 0 has no output written.
+// Scratch of the parts that shared_merge_kernel joins; m in powers of two, and a part with l = 0 has
+// no output written.
 struct SharedParts {
+    // of the 128-row kernel: [T][n_heads][n][hd] outputs and [T][n_heads][n] (m, l)
     float* o;
     float2* ml;
     int n;
     int direct;  // no scratch and no merge
+    // of the 16-row kernel: share w's piece of unit u has place w + u (unique: each piece after a
+    // share's first, and each share after the first, raises one of the two): [places][n_kv][16][hd]
+    // and [places][n_kv][16]; of every unit the first share that has a piece, and how many do
+    float* po;
+    float2* pml;
+    int2* unit;
 };
 
 // Rows of request `req` at or past max_q (no tile holds them): NaN, in the heads of one KV head.

@@ -519,15 +519,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!parts.direct) {
             if (group == last && r < rows) parts.ml[static_cast<size_t>(row) * parts.n + split] = make_float2(m, l);
             if (nb > 0) {
-                float* dst = parts.o + (static_cast<size_t>(row) * parts.n + split) * HD;
+                // Through the ring, whose copies and products are done, so that a warp writes whole
+                // rows: stored from the registers, a row a lane, they took three times as long.
+                constexpr int kPitch = HD * 4 + 16;  // lanes' rows start in different banks
+                static_assert(kRows * kPitch <= S::kOffP, "the output fits where the ring was");
 #pragma unroll 1
                 for (int col = group * (HD / 2); col < (group + 1) * (HD / 2); col += 32) {
                     uint32_t o[32];
                     tmem_ld_32x32b_x32(tmem_o + lane_off + col, o);
                     tmem_ld_wait();
-                    if (r < rows) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) st_v8(dst + col + 8 * i, o + 8 * i);
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(sm + r * kPitch + col * 4 + 16 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+                if (group == 0) s_pos[r] = row;  // positions are no longer read
+                asm volatile("bar.sync 13, 256;" ::: "memory");  // the softmax warps
+                constexpr int kLanes = HD / 4 < 32 ? HD / 4 : 32, kAt = 32 / kLanes;  // lanes of a row, rows at once
+                for (int q = warp * kAt + lane / kLanes; q < rows; q += kSoftWarps * kAt) {
+                    float* dst = parts.o + (static_cast<size_t>(s_pos[q]) * parts.n + split) * HD;
+#pragma unroll
+                    for (int i = 0; i < HD / 4 / kLanes; ++i) {
+                        const int at = (lane % kLanes + i * kLanes) * 4;
+                        *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(sm + q * kPitch + at * 4);
                     }
                 }
             }

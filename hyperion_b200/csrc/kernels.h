@@ -372,6 +372,7 @@ struct SharedAttnParams {
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
 };
+constexpr int kMaxSharedRequests = 1024;
 size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
                                  int hd);
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream);

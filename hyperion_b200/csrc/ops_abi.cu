@@ -472,7 +472,7 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
 
 static bool shared_shape_ok(int32_t T, int32_t n_req, int32_t max_q, int32_t max_own, int32_t prefix_len,
                             int32_t n_heads, int32_t n_kv) {
-    return T >= 1 && n_req >= 1 && max_q >= 1 && max_own >= 0 && prefix_len >= 0 && n_kv >= 1 && n_heads >= 1 &&
+    return T >= 1 && n_req >= 1 && n_req <= hyb::kMaxSharedRequests && max_q >= 1 && max_own >= 0 && prefix_len >= 0 && n_kv >= 1 && n_heads >= 1 &&
            n_heads % n_kv == 0 && static_cast<int64_t>(T) * n_heads <= INT32_MAX - 64 && static_cast<int64_t>(prefix_len) + max_own <= INT32_MAX - 65536;
 }
 

@@ -292,10 +292,11 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   not matter before or after). Rows at or past max_q of a request, and rows of a request
  *   with more than max_own or max_blocks * page_size keys, become NaN; so do rows some of
  *   whose tile of rows read a page outside [0, n_pages). A negative own_lens counts as 0.
- *   Slots that no row of the call sees may hold anything (NaN included); the ones that some
- *   row sees must be finite.
- * head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; n_pages * page_size < 2^31;
- * q, the pools, out and scratch 16-byte aligned.
+ *   A request's rows are taken to stand at neighbouring positions: slots before the first and
+ *   after the last key that its rows see may hold anything (NaN included), those between
+ *   must be finite.
+ * n_req is 1..1024; head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; n_pages *
+ * page_size < 2^31; q, the pools, out and scratch 16-byte aligned.
  */
 size_t hyb_sdpa_shared_prefix_scratch_bytes(int32_t T, int32_t n_req, int32_t max_q, int32_t max_own,
                                             int32_t prefix_len, int32_t n_heads, int32_t n_kv, int32_t head_dim);

@@ -53,7 +53,7 @@ def _attn(L, **kw):
     return L.hyb_sdpa_shared_prefix(*a.values(), None)
 
 
-@pytest.mark.parametrize("kw", [dict(q=None), dict(scratch=None), dict(pt=None), dict(T=0), dict(n_req=0), dict(max_q=0),
+@pytest.mark.parametrize("kw", [dict(q=None), dict(scratch=None), dict(pt=None), dict(T=0), dict(n_req=0), dict(n_req=1025), dict(max_q=0),
                                 dict(max_own=-1), dict(plen=-1), dict(H=3, nkv=2), dict(window=-1), dict(n_pages=0),
                                 dict(max_blocks=0), dict(n_pages=1 << 28), dict(q=ODD), dict(out=ODD), dict(scratch=ODD),
                                 dict(plen=(1 << 31) - 1), dict(nbytes=64)])

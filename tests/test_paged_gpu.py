@@ -359,6 +359,20 @@ def test_attn_many_blocks(built_lib, hd):
     b.check(b.call(), rows=[0, 63])
 
 
+@pytest.mark.parametrize("n,window", [(300, 0), (1024, 0), (257, 20)])
+@pytest.mark.parametrize("prefix", [0, 70, 700])
+def test_attn_many_requests(built_lib, n, window, prefix):
+    """Requests without rows, without keys, with one key and with hundreds, in shares that cross them."""
+    rng = np.random.default_rng(n + prefix)
+    own = rng.choice([0, 0, 1, 5, 16, 17, 40, 300], n)
+    q = np.where(rng.random(n) < 0.2, 0, 1 + (rng.random(n) < 0.1))
+    q[:3], own[:3] = 0, 50
+    b = Batch(4, 2, 64, 16, prefix, own, q, seed=n, window=window, pad_rows=2)
+    got = b.call()
+    b.check(got, rows=sorted(rng.choice(b.T - 2, 60, replace=False).tolist()) + [b.T - 3])
+    assert (got[-2:] == 7.0).all()
+
+
 def test_attn_scores_far_apart(built_lib):
     """Scores of some hundreds, growing along the keys (every tile moves the maximum) and falling."""
     for order in (1, -1):

@@ -45,56 +45,91 @@ constexpr int kSlice = 16;  // keys of one warp step
 constexpr int kMinSlices = 4;     // of a warp's share: a shorter one is all latency
 constexpr int kCtas = 2 * 148;    // two on every SM of a B200
 
-SharedPlan plan_shared(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv, int hd, int window) {
+// The sizes of a call that the plan goes by.
+struct Sizes {
+    int T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd;
+    long long all_rows, req_rows;  // (token, head) pairs of a KV head: of all rows, of a request's
+    int tiles_o, tc_tiles, tc_tiles_o;
+    Sizes(int T_, int n_req_, int max_q_, int max_own_, int prefix_len_, int n_heads_, int n_kv_, int hd_)
+        : T(T_), n_req(n_req_), max_q(std::min(max_q_, T_)), max_own(max_own_), prefix_len(prefix_len_), n_heads(n_heads_),
+          n_kv(n_kv_), hd(hd_) {
+        const int G = n_heads / n_kv;
+        auto tiles = [](long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); };
+        all_rows = static_cast<long long>(T) * G;
+        req_rows = static_cast<long long>(max_q) * G;
+        tiles_o = tiles(req_rows, kTileRows);
+        tc_tiles = tiles(all_rows, kTcRows);
+        tc_tiles_o = tiles(req_rows, kTcRows);
+    }
+    // keys of the prefix, and 64-key blocks of prefix and own keys, that one row sees at most
+    long long seen(int window) const { return window > 0 ? std::min(prefix_len, window) : prefix_len; }
+    long long blocks(int window) const {
+        const long long all = static_cast<long long>(prefix_len) + max_own;
+        return ((window > 0 ? std::min<long long>(all, static_cast<long long>(window) + max_q) : all) + 63) / 64;
+    }
+};
+
+// The ways to go through a call's keys.
+enum class Way {
+    kApart,       // the prefix by tiles of all rows, the requests' own keys by the 16-row kernel
+    kPerRequest,  // 128-row tiles of one request's rows over prefix and own keys
+    kTogether,    // the 16-row kernel over both
+};
+
+// The only sensible one, where there is one.
+bool only_way(const Sizes& z, Way* way) {
+    // up to 16 rows in all: one 16-row tile of them against the prefix, unless there is nobody to share with
+    if (z.all_rows <= kTileRows) *way = z.prefix_len > 128 && z.n_req > 1 ? Way::kApart : Way::kTogether;
+    // tiles of one request's rows that are filled about as well as those of all rows
+    else if (z.req_rows > kTileRows && 4ll * z.n_req * z.tc_tiles_o <= 5ll * z.tc_tiles) *way = Way::kPerRequest;
+    else if (z.prefix_len == 0) *way = Way::kTogether;
+    else return false;
+    return true;
+}
+
+// Otherwise by what they take, in microseconds (the constants as measured).
+Way way_of(const Sizes& z, int window) {
+    Way way;
+    if (only_way(z, &way)) return way;
+    // 128-row kernel: 8 to start and end and a block on an SM 0.8, with head_dim 256 1.2; 16-row kernel: 5, and
+    // slices of head_dim 256 at 400 in a microsecond from HBM, 650 when read again (L2); joining: 6; the two
+    // kernels one after the other: 8. Half of max_own stands for the requests' mean.
+    const double wide = z.hd / 256., block = 0.4 + 0.8 * wide;
+    const double units_o = static_cast<double>(z.n_req) * z.tiles_o * z.n_kv, own = units_o * z.max_own / 2 / kSlice * wide / 400;
+    const long long units_tc = static_cast<long long>(z.n_req) * z.tc_tiles_o * z.n_kv, seen = z.seen(window);
+    const double per_request = 8 + static_cast<double>((units_tc + 147) / 148 * z.blocks(window)) * block;
+    const double together = 11 + own + units_o * static_cast<double>(seen / kSlice) * wide / 650;
+    const double apart = 27 + own + std::max(1., static_cast<double>(z.tc_tiles * z.n_kv * ((seen + 63) / 64)) / 148) * block;
+    if (per_request < together && per_request < apart) return Way::kPerRequest;
+    return together < apart ? Way::kTogether : Way::kApart;
+}
+
+SharedPlan plan_of(const Sizes& z, Way way, int window) {
     SharedPlan s;
-    const int G = n_heads / n_kv;
-    max_q = std::min(max_q, T);
-    const long long all_rows = static_cast<long long>(T) * G, req_rows = static_cast<long long>(max_q) * G;
-    auto tiles = [](long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); };
-    // Tiles of one request's rows when they fill 128-row tiles about as well as the whole
-    // batch's rows do: then prefix and own keys are one pass.
-    if (req_rows > kTileRows && 4ll * n_req * tiles(req_rows, kTcRows) <= 5ll * tiles(all_rows, kTcRows)) {
+    if (way == Way::kPerRequest) {
+        const long long units = static_cast<long long>(z.n_req) * z.tc_tiles_o * z.n_kv;
         s.tc_per_request = 1;
-        s.tc_tiles = tiles(req_rows, kTcRows);
-        const long long units = static_cast<long long>(s.tc_tiles) * n_kv * n_req;
-        const long long blocks = (static_cast<long long>(prefix_len) + max_own + 63) / 64;
-        s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((blocks + 1) / 2, 148 / units)));
+        s.tc_tiles = z.tc_tiles_o;
+        s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((z.blocks(window) + 1) / 2, 148 / units)));
         return s;
     }
-    const int tiles_o = tiles(req_rows, kTileRows);
-    const long long units_o = static_cast<long long>(n_req) * tiles_o * n_kv;
-    const long long seen = window > 0 ? std::min(prefix_len, window) : prefix_len;  // of the prefix, by one row at most
-    if (prefix_len > 0) {
-        // The prefix apart, read once for all rows, or again for every request (from L2) in one go with
-        // its own keys? The 16-row kernel gets through some 650 slices of head_dim 256 in a
-        // microsecond then (L2's rate); the 128-row kernel takes about 10 us to start, end and be joined
-        // and 1.2 us a block of head_dim 256 on each SM. A single request shares with nobody.
-        const double again = static_cast<double>(units_o) * ((seen + kSlice - 1) / kSlice) * hd / (256 * 650.);
-        const int tc_tiles = tiles(all_rows, kTcRows);
-        const double apart = 10 + 1.2 * std::max(1., static_cast<double>(tc_tiles) * n_kv * ((seen + 63) / 64) / 148) * hd / 256;
-        if (all_rows <= kTileRows) s.o_prefix = n_req == 1 || prefix_len <= 128;
-        else s.o_prefix = again < apart;
-        if (!s.o_prefix) {
-            if (all_rows <= kTileRows) {
-                s.prefix_unit = 1;
-            } else {
-                s.tc_tiles = tc_tiles;
-                const long long units = static_cast<long long>(tc_tiles) * n_kv;
-                s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((seen + 127) / 128, 148 / units)));
-            }
-        }
+    if (way == Way::kApart && z.all_rows > kTileRows) {
+        const long long units = static_cast<long long>(z.tc_tiles) * z.n_kv;
+        s.tc_tiles = z.tc_tiles;
+        s.tc_splits = static_cast<int>(std::max<long long>(1, std::min<long long>((z.seen(window) + 127) / 128, 148 / units)));
     }
-    const long long unit_slices = (max_own + kSlice - 1) / kSlice + (s.o_prefix ? (prefix_len + kSlice - 1) / kSlice : 0);
-    if (unit_slices > 0) s.tiles_o = tiles_o;
-    if (s.tiles_o > 0 && s.tc_tiles == 0 && s.prefix_unit == 0 && unit_slices <= 4 * kMinSlices) {
+    s.prefix_unit = way == Way::kApart && z.all_rows <= kTileRows;
+    s.o_prefix = way == Way::kTogether && z.prefix_len > 0;
+    const long long prefix_slices = (z.prefix_len + kSlice - 1) / kSlice;
+    const long long unit_slices = (z.max_own + kSlice - 1) / kSlice + (s.o_prefix ? prefix_slices : 0);
+    if (unit_slices > 0) s.tiles_o = z.tiles_o;
+    if (way == Way::kTogether && unit_slices > 0 && unit_slices <= kWarps * kMinSlices) {
         s.one_part = 1;
         return s;
     }
-    const long long slices = (s.tiles_o > 0 ? units_o * unit_slices : 0) + static_cast<long long>(s.prefix_unit) * n_kv * ((prefix_len + kSlice - 1) / kSlice);
-    // as many shares of every KV head as fill two CTAs an SM
-    const long long head_slices = slices / n_kv;
-    s.shares = static_cast<int>(std::max<long long>(1, std::min<long long>(kCtas * kWarps / n_kv, head_slices / kMinSlices)));
-    if (slices == 0) s.shares = 0;
+    // as many shares of every KV head's slices as fill two CTAs an SM
+    const long long slices = static_cast<long long>(z.n_req) * s.tiles_o * unit_slices + (s.prefix_unit ? prefix_slices : 0);
+    if (slices > 0) s.shares = static_cast<int>(std::max<long long>(1, std::min<long long>(kCtas * kWarps / z.n_kv, slices / kMinSlices)));
     return s;
 }
 
@@ -732,15 +767,17 @@ void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, const Shar
 
 size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int prefix_len, int n_heads, int n_kv,
                                  int hd) {
-    // For any window: the prefix apart takes most without one (the most parts), together with the
-    // requests' keys the same with any, and the shorter the window the sooner they go together.
-    const SharedPlan none = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd, 0);
-    const SharedPlan least = plan_shared(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd, 1);
-    return std::max(Layout(none, T, n_req, n_heads, n_kv, hd).bytes, Layout(least, T, n_req, n_heads, n_kv, hd).bytes) + 512;
+    // For any window: the most that a way takes, which is without one (the most keys, so the most parts).
+    const Sizes z(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd);
+    auto bytes = [&](Way way) { return Layout(plan_of(z, way, 0), T, n_req, n_heads, n_kv, hd).bytes; };
+    Way way;
+    const size_t most = only_way(z, &way) ? bytes(way) : std::max({bytes(Way::kApart), bytes(Way::kPerRequest), bytes(Way::kTogether)});
+    return most + 512;
 }
 
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
-    const SharedPlan pl = plan_shared(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd, p.window);
+    const Sizes z(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd);
+    const SharedPlan pl = plan_of(z, way_of(z, p.window), p.window);
     const Layout at(pl, p.T, p.n_req, p.n_heads, p.n_kv, p.hd);
     if (p.scratch_bytes < at.bytes + 512) throw ArgError("sdpa_shared_prefix: scratch too small");
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p.scratch) + 255) & ~static_cast<uintptr_t>(255));

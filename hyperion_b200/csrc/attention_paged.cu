@@ -199,8 +199,9 @@ struct SmallPlan {
 // Neighbouring warps take the same share for neighbouring heads, whose keys are neighbours in
 // memory: with the heads one after the other in the row of slices the same kernel reached half
 // the bandwidth. ONE: short units, a CTA takes a whole one, joins its four warps and writes
-// the output itself.
-template <int HD, bool ONE>
+// the output itself. PLAIN: no soft-cap and a positive scale, so that a row's maximum is that of its
+// raw products.
+template <int HD, bool ONE, bool PLAIN>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     shared_attn_small_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                              const SharedAttnParams p, const SharedPlan pl, SharedParts parts, int after_tc) {
@@ -422,8 +423,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     };
 #pragma unroll
     for (int j = 0; j < ST - 1; ++j) fetch(j);
-    const bool plain = p.softcap <= 0.f && p.scale > 0.f;  // the maximum is taken over the raw products
-    const float s2 = plain ? p.scale * kSharedLog2e : 1.f;
+    const float s2 = PLAIN ? p.scale * kSharedLog2e : 1.f;
     // ldmatrix offsets of this lane in a [16 keys][128 bytes] box, for the four 32-byte columns
     uint32_t k_off[4], v_off[4];
     {
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             v[4] = s0v[2], v[5] = s0v[3], v[6] = s1v[2], v[7] = s1v[3];
             if (++slot == ST) slot = 0, phase ^= 1;
         }
-        if (!plain) {
+        if constexpr (!PLAIN) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 v[j] = kSharedLog2e * (p.softcap > 0.f ? p.softcap * tanhf(v[j] * p.scale / p.softcap) : v[j] * p.scale);
@@ -751,7 +751,9 @@ void launch_shared_t(const SharedAttnParams& p, const SharedPlan& pl, const Shar
         if (ctas > INT_MAX / kTileRows) throw ArgError("sdpa_shared_prefix: too many rows");
         CUtensorMap tk, tv;
         shared_pool_maps(p, kSlice, &tk, &tv);
-        auto kern = pl.one_part ? shared_attn_small_kernel<HD, true> : shared_attn_small_kernel<HD, false>;
+        const bool plain = p.softcap <= 0.f && p.scale > 0.f;
+        auto kern = pl.one_part ? (plain ? shared_attn_small_kernel<HD, true, true> : shared_attn_small_kernel<HD, true, false>)
+                                : (plain ? shared_attn_small_kernel<HD, false, true> : shared_attn_small_kernel<HD, false, false>);
         allow_smem(reinterpret_cast<const void*>(kern), SP::kSmem);
         shared_launch(kern, static_cast<unsigned>(ctas), kWarps * 32, SP::kSmem, stream,
                       pl.tc_splits > 0, tk, tv, p, pl, parts, pl.tc_splits > 0 ? 1 : 0);

@@ -1,7 +1,8 @@
 // Shared-prefix attention for many rows on the 5th-generation tensor cores: the part of
 // attention_paged.cu's work whose rows fill a 128-row tile.
 //
-// One CTA: 128 (token, head) rows of one KV head against a run of 64-key blocks. The rows are
+// One CTA: 128 (token, head) rows of one KV head against a run of key blocks (of 128 keys; of 64
+// at head_dim 256). The rows are
 // those of the whole batch against the prefix (decode), or those of one request against the
 // prefix and then its own keys (prefill). One pass over the keys with a running maximum:
 //   S = Q K^T (tcgen05.mma, fp32 in TMEM, two buffers), p = exp2(s - m) into a bf16 operand
@@ -17,7 +18,7 @@
 //   hands the rows' references on to the other before it starts its exponentials.
 // Warps 8 and 9: producers of the K and of the V blocks. They look the pages up (32 table
 //   entries at a time, one a lane, a batch ahead) and issue the tensor-map copies: boxes of 64
-//   head_dim columns of min(page_size, 64) slots, 128-byte swizzled.
+//   head_dim columns of min(page_size, block) slots, 128-byte swizzled.
 // Warp 10: allocates TMEM and issues the MMAs from one lane, S(c + 2) before P V(c), so that
 //   the softmax of a block runs under the products of its neighbours.
 // In the few blocks that stick out of the visible keys the softmax group clears the V rows
@@ -37,7 +38,6 @@ __device__ int g_shared_attn_wait_timeouts = 0;
 namespace {
 
 constexpr int kRows = kTcRows;  // 128
-constexpr int kKeys = 64;
 constexpr int kSoftWarps = 8;
 constexpr int kGroupWarps = 4;
 constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 2;  // two producers: K, V
@@ -48,11 +48,14 @@ constexpr int kThreads = kSoftWarps * 32 + 96;
 // head_dim 256, where shared memory is what the kernel saturates).
 template <int HD>
 struct TcShared {
-    static constexpr uint32_t kTmemCols = HD == 64 ? 256 : 512;  // S 2 x 64, O HD, Q HD / 2
+    // keys of a block: 128 where TMEM holds two such S beside O (a block's waits, commits and hand-overs
+    // cost the same whatever its length: 1780 cycles for 64 keys of head_dim 128)
+    static constexpr int kKeys = HD == 256 ? 64 : 128;
+    static constexpr uint32_t kTmemCols = 512;  // S 2 x kKeys, O HD, Q HD / 2
     static constexpr int kSub = HD / 64;
-    static constexpr int kSlots = HD == 256 ? 6 : 12;
+    static constexpr int kSlots = HD == 256 ? 6 : (HD == 128 ? 5 : 8);
     static constexpr int kTileBytes = kKeys * HD * 2;
-    static constexpr int kPBytes = kRows * kKeys * 2;
+    static constexpr int kPBytes = kRows * kKeys * 2;  // kKeys / 64 sub-tiles of [128 rows][128 bytes]
     static constexpr int kOffP = kSlots * kTileBytes;
     static constexpr int kOffSum = kOffP;                    // float [kRows], once P is no longer read
     static constexpr int kOffRef = kOffP + 2 * kPBytes;      // float [kRows]: the rows' references
@@ -126,12 +129,12 @@ __device__ __forceinline__ void st_v8(float* p, const uint32_t* r) {
                  : "memory");
 }
 
-// The keys of one segment (prefix or own) that a tile of rows sees: [lo, hi), in 64-key blocks.
+// The keys of one segment (prefix or own) that a tile of rows sees: [lo, hi), in blocks from `first` on.
 struct Segment {
     const int* table;
-    int base, lo, hi, blocks;
-    __device__ int first() const { return lo & ~(kKeys - 1); }
+    int base, lo, hi, first, blocks;
 };
+template <int kKeys>
 __device__ __forceinline__ Segment segment(const int* table, int base, int len, int pmin, int pmax, int window) {
     Segment s;
     s.table = table;
@@ -140,16 +143,18 @@ __device__ __forceinline__ Segment segment(const int* table, int base, int len, 
     s.lo = window > 0 && pmax >= 0
                ? static_cast<int>(min(static_cast<long long>(s.hi), max(0ll, static_cast<long long>(pmin) - window + 1 - base)))
                : 0;
-    s.blocks = s.hi > s.lo ? (s.hi - s.first() + kKeys - 1) / kKeys : 0;
+    s.first = s.lo & ~(kKeys - 1);
+    s.blocks = s.hi > s.lo ? (s.hi - s.first + kKeys - 1) / kKeys : 0;
     return s;
 }
 
-template <int HD>
+// PLAIN: no soft-cap and a positive scale, so that a row's maximum is that of its raw products.
+template <int HD, bool PLAIN>
 __global__ void __launch_bounds__(kThreads, 1)
     shared_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                           const SharedAttnParams p, const SharedPlan pl, SharedParts parts) {
     using S = TcShared<HD>;
-    constexpr int SUB = S::kSub, SLOTS = S::kSlots;
+    constexpr int SUB = S::kSub, SLOTS = S::kSlots, kKeys = S::kKeys, HALVES = kKeys / 64;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* sm = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
     const uint32_t sbase = smem_u32(sm);
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const uint32_t tmem_s = tmem, tmem_o = tmem + 128, tmem_q = tmem_o + HD;
+    const uint32_t tmem_s = tmem, tmem_o = tmem + 2 * kKeys, tmem_q = tmem_o + HD;
 
     int pmin = INT_MAX, pmax = -1;
     for (int i = lane; i < kRows; i += 32)
@@ -256,9 +261,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     pmin = __reduce_min_sync(0xffffffffu, pmin);
     pmax = __reduce_max_sync(0xffffffffu, pmax);
-    const Segment sp = segment(p.prefix_table, 0, p.prefix_len, pmin, pmax, p.window);
-    Segment so = {nullptr, p.prefix_len, 0, 0, 0};
-    if (per_request) so = segment(p.table + static_cast<size_t>(req) * p.max_blocks, p.prefix_len, own, pmin, pmax, p.window);
+    const Segment sp = segment<kKeys>(p.prefix_table, 0, p.prefix_len, pmin, pmax, p.window);
+    Segment so = {nullptr, p.prefix_len, 0, 0, 0, 0};
+    if (per_request) so = segment<kKeys>(p.table + static_cast<size_t>(req) * p.max_blocks, p.prefix_len, own, pmin, pmax, p.window);
     const int all = sp.blocks + so.blocks;
     const int c0 = static_cast<int>(static_cast<long long>(all) * split / pl.tc_splits);
     const int nb = __shfl_sync(0xffffffffu, static_cast<int>(static_cast<long long>(all) * (split + 1) / pl.tc_splits) - c0, 0);
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b = c0 + c;
         const bool own = b >= sp.blocks;
         const Segment& s = own ? so : sp;
-        key0 = s.first() + (own ? b - sp.blocks : b) * kKeys;
+        key0 = s.first + (own ? b - sp.blocks : b) * kKeys;
         return s;
     };
     bool ok = true;
@@ -330,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t lo = (ring + slot * (S::kTileBytes >> 4)) | (1u << 16);
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
-                mma_tmem_a(tmem_s + 64 * sb, tmem_q + 8 * kk, lo + (kk >> 2) * (kKeys * 128 >> 4) + 2 * (kk & 3), id_s, kk > 0, leader);
+                mma_tmem_a(tmem_s + kKeys * sb, tmem_q + 8 * kk, lo + (kk >> 2) * (kKeys * 128 >> 4) + 2 * (kk & 3), id_s, kk > 0, leader);
             commit_if(s_full + 8 * sb, leader);
             commit_if(slot_empty + 8 * slot, leader);
         };
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t vlo = (ring + vs * (S::kTileBytes >> 4)) | (((kKeys * 128 >> 4) & 0x3FFFu) << 16);
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
-                    mma_smem_a(tmem_o, p_lo + sb * (S::kPBytes >> 4) + 2 * kk, vlo + kk * (2048 >> 4), id_o, c > 0 || kk > 0, leader);
+                    mma_smem_a(tmem_o, p_lo + sb * (S::kPBytes >> 4) + (kk >> 2) * (kRows * 128 >> 4) + 2 * (kk & 3), vlo + kk * (2048 >> 4), id_o, c > 0 || kk > 0, leader);
                 commit_if(pv_done + 8 * sb, leader);
                 commit_if(slot_empty + 8 * vs, leader);
                 vs += c + 2 < nb ? 2 : 1;
@@ -388,9 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
         const int mine = 1 + 2 * quad + group, other = 1 + 2 * quad + (group ^ 1);  // hand-over barriers
-        // with a plain positive scale the maximum is taken over the raw products
-        const bool plain = p.softcap <= 0.f && p.scale > 0.f;
-        const float s2 = plain ? p.scale * kSharedLog2e : 1.f;
+        const float s2 = PLAIN ? p.scale * kSharedLog2e : 1.f;
         float m = -INFINITY;  // the reference that l is held at
         float l = 0.f;
         for (int c = group; c < nb; c += 2) {
@@ -398,36 +401,46 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Segment& s = block(c, key0);
             wait_b(ok, s_full + 8 * group, (c >> 1) & 1);
             tc_fence_after();
-            uint32_t v[2][32];
-            tmem_ld_32x32b_x32(tmem_s + lane_off + 64 * group, v[0]);
-            tmem_ld_32x32b_x32(tmem_s + lane_off + 64 * group + 32, v[1]);
-            tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty + 8 * group);
-            float x[64];
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]);
-            if (!plain) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    x[i] = kSharedLog2e * (p.softcap > 0.f ? p.softcap * tanhf(x[i] * p.scale / p.softcap) : x[i] * p.scale);
-            }
             // blocks wholly inside every row's view skip the per-key mask
             const bool full = key0 >= s.lo && key0 + kKeys <= s.hi && s.base + key0 + kKeys - 1 <= pmin &&
                               (p.window == 0 || s.base + key0 > pmax - p.window);
-            if (!full) {
-                const long long wlo = p.window > 0 ? static_cast<long long>(pos) - p.window + 1 - s.base : 0;
-                const int from = static_cast<int>(min(max(wlo, static_cast<long long>(s.lo)), static_cast<long long>(s.hi))) - key0;
-                const int to = min(s.hi - 1, pos - s.base) + 1 - key0;
+            const long long wlo = p.window > 0 ? static_cast<long long>(pos) - p.window + 1 - s.base : 0;
+            const int from = static_cast<int>(min(max(wlo, static_cast<long long>(s.lo)), static_cast<long long>(s.hi))) - key0;
+            const int to = min(s.hi - 1, pos - s.base) + 1 - key0;
+            float x[64];
+            auto load = [&](int h) {  // the scores of the block's keys 64 h .. 64 h + 63
+                uint32_t v[2][32];
+                tmem_ld_32x32b_x32(tmem_s + lane_off + kKeys * group + 64 * h, v[0]);
+                tmem_ld_32x32b_x32(tmem_s + lane_off + kKeys * group + 64 * h + 32, v[1]);
+                tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (i < from || i >= to) x[i] = -INFINITY;
+                for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]);
+                if constexpr (!PLAIN) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        x[i] = kSharedLog2e * (p.softcap > 0.f ? p.softcap * tanhf(x[i] * p.scale / p.softcap) : x[i] * p.scale);
+                }
+                if (!full) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (64 * h + i < from || 64 * h + i >= to) x[i] = -INFINITY;
+                }
+            };
+            auto read = [&]() {  // S is free for block c + 2
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty + 8 * group);
+            };
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int h = 0; h < HALVES; ++h) {
+                load(h);
+                if (HALVES == 1) read();
+                float mx4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int i = 4; i < 64; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], x[i]);
+                mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * s2);
             }
-            float mx4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-            for (int i = 4; i < 64; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], x[i]);
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * s2;
             // the reference after block c - 1, moved if this block outgrows it, for block c + 1
             float ref = -INFINITY;
             if (c > 0) {
@@ -465,20 +478,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l *= shared_ex2(m - z);  // 0 * 0 where nothing was seen yet
                 m = now;
             }
-            uint32_t w[32];
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            // one half is still in registers; of two, both are read again (keeping one spills)
+#pragma unroll 1
+            for (int h = 0; h < HALVES; ++h) {
+                if (HALVES > 1) {
+                    load(h);
+                    if (h + 1 == HALVES) read();
+                }
+                uint32_t w[32];
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                w[i] = shared_pack(shared_ex2(fmaf(x[2 * i], s2, -z)), shared_ex2(fmaf(x[2 * i + 1], s2, -z)));
-                sum[(2 * i) & 3] += __uint_as_float(w[i] << 16);
-                sum[(2 * i + 1) & 3] += __uint_as_float(w[i] & 0xffff0000u);
+                for (int i = 0; i < 32; ++i) {
+                    w[i] = shared_pack(shared_ex2(fmaf(x[2 * i], s2, -z)), shared_ex2(fmaf(x[2 * i + 1], s2, -z)));
+                    sum[(2 * i) & 3] += __uint_as_float(w[i] << 16);
+                    sum[(2 * i + 1) & 3] += __uint_as_float(w[i] & 0xffff0000u);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (h == 0 && c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);  // the buffer's last reader
+                unsigned char* prow = sm + S::kOffP + group * S::kPBytes + h * (kRows * 128) + r * 128;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    *reinterpret_cast<uint4*>(prow + ((i ^ (r & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if (c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);  // the buffer's last reader
-            unsigned char* prow = sm + S::kOffP + group * S::kPBytes + r * 128;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<uint4*>(prow + ((i ^ (r & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
             if (key0 < s.lo || key0 + kKeys > s.hi) {
                 // V rows that no row of the tile sees; the block's V has its place in the ring to
                 // itself until P V(c), and what held the place before was used up by a product
@@ -588,11 +609,12 @@ template <int HD>
 void launch_t(const SharedAttnParams& p, const SharedPlan& pl, const SharedParts& parts, cudaStream_t stream) {
     using S = TcShared<HD>;
     CUtensorMap tk, tv;
-    shared_pool_maps(p, p.page_size < kKeys ? p.page_size : kKeys, &tk, &tv);
-    allow_smem(reinterpret_cast<const void*>(shared_attn_tc_kernel<HD>), S::kSmem);
+    shared_pool_maps(p, p.page_size < S::kKeys ? p.page_size : S::kKeys, &tk, &tv);
+    auto kern = p.softcap <= 0.f && p.scale > 0.f ? shared_attn_tc_kernel<HD, true> : shared_attn_tc_kernel<HD, false>;
+    allow_smem(reinterpret_cast<const void*>(kern), S::kSmem);
     const long long ctas = static_cast<long long>(pl.tc_tiles) * (pl.tc_per_request ? p.n_req : 1) * p.n_kv * pl.tc_splits;
     if (ctas > INT_MAX) throw ArgError("sdpa_shared_prefix: too many parts");
-    shared_attn_tc_kernel<HD><<<static_cast<unsigned>(ctas), kThreads, S::kSmem, stream>>>(tk, tv, p, pl, parts);
+    kern<<<static_cast<unsigned>(ctas), kThreads, S::kSmem, stream>>>(tk, tv, p, pl, parts);
     HYB_LAUNCH_CHECK("shared_attn_tc_kernel");
 }
 

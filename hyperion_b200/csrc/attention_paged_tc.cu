@@ -53,11 +53,15 @@ struct TcShared {
     static constexpr int kKeys = HD == 256 ? 64 : 128;
     static constexpr uint32_t kTmemCols = 512;  // S 2 x kKeys, O HD, Q HD / 2
     static constexpr int kSub = HD / 64;
-    static constexpr int kSlots = HD == 256 ? 6 : (HD == 128 ? 5 : 8);
+    // P: at head_dim 256 in TMEM, over the S it comes from (a quarter of the shared-memory traffic less,
+    // which is what bounds the kernel there: 2160 -> 1700 cycles a block), S(c + 2) then follows
+    // P V(c); otherwise in shared memory, and S(c + 2) goes first
+    static constexpr bool kPTmem = HD == 256;
+    static constexpr int kSlots = HD == 256 ? 7 : (HD == 128 ? 5 : 8);
     static constexpr int kTileBytes = kKeys * HD * 2;
-    static constexpr int kPBytes = kRows * kKeys * 2;  // kKeys / 64 sub-tiles of [128 rows][128 bytes]
+    static constexpr int kPBytes = kPTmem ? 0 : kRows * kKeys * 2;  // kKeys / 64 sub-tiles of [128 rows][128 bytes]
     static constexpr int kOffP = kSlots * kTileBytes;
-    static constexpr int kOffSum = kOffP;                    // float [kRows], once P is no longer read
+    static constexpr int kOffSum = kOffP - kRows * 4;        // float [kRows], once the ring is no longer read
     static constexpr int kOffRef = kOffP + 2 * kPBytes;      // float [kRows]: the rows' references
     static constexpr int kOffPos = kOffRef + kRows * 4;      // int [kRows]: positions
     static constexpr int kOffBars = kOffPos + kRows * 4;
@@ -350,29 +354,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // S(c + 2) goes before P V(c): its buffer is free as soon as the softmax of block c has
             // read it, and the group finds it ready when it is through with block c
+            auto next_s = [&]() {
+                ks += 2;
+                if (ks >= SLOTS) {
+                    ks -= SLOTS;
+                    kph ^= 1;
+                }
+            };
             for (int c = 0; c < nb; ++c) {
                 const int sb = c & 1;
                 const bool v_here = shared_try_wait(slot_full + 8 * vs, vph);  // asked for ahead of its use
+                bool k_here = true;
                 if (c + 2 < nb) {
-                    ks += 2;
-                    if (ks >= SLOTS) {
-                        ks -= SLOTS;
-                        kph ^= 1;
+                    next_s();
+                    k_here = shared_try_wait(slot_full + 8 * ks, kph);
+                    if constexpr (!S::kPTmem) {
+                        warp_wait(ok, s_empty + 8 * sb, (c >> 1) & 1);
+                        if (!__all_sync(0xffffffffu, k_here)) warp_wait(ok, slot_full + 8 * ks, kph);
+                        issue_s(sb, ks);
                     }
-                    const bool k_here = shared_try_wait(slot_full + 8 * ks, kph);
-                    warp_wait(ok, s_empty + 8 * sb, (c >> 1) & 1);
-                    if (!__all_sync(0xffffffffu, k_here)) warp_wait(ok, slot_full + 8 * ks, kph);
-                    issue_s(sb, ks);
                 }
                 if (!__all_sync(0xffffffffu, v_here)) warp_wait(ok, slot_full + 8 * vs, vph);
                 warp_wait(ok, p_full + 8 * sb, (c >> 1) & 1);
                 tc_fence_after();
                 const uint32_t vlo = (ring + vs * (S::kTileBytes >> 4)) | (((kKeys * 128 >> 4) & 0x3FFFu) << 16);
 #pragma unroll
-                for (int kk = 0; kk < kKeys / 16; ++kk)
-                    mma_smem_a(tmem_o, p_lo + sb * (S::kPBytes >> 4) + (kk >> 2) * (kRows * 128 >> 4) + 2 * (kk & 3), vlo + kk * (2048 >> 4), id_o, c > 0 || kk > 0, leader);
+                for (int kk = 0; kk < kKeys / 16; ++kk) {
+                    if constexpr (S::kPTmem)
+                        mma_tmem_a(tmem_o, tmem_s + kKeys * sb + 8 * kk, vlo + kk * (2048 >> 4), id_o, c > 0 || kk > 0, leader);
+                    else
+                        mma_smem_a(tmem_o, p_lo + sb * (S::kPBytes >> 4) + (kk >> 2) * (kRows * 128 >> 4) + 2 * (kk & 3),
+                                   vlo + kk * (2048 >> 4), id_o, c > 0 || kk > 0, leader);
+                }
                 commit_if(pv_done + 8 * sb, leader);
                 commit_if(slot_empty + 8 * vs, leader);
+                if constexpr (S::kPTmem) {
+                    // MMAs run in order: S(c + 2) overwrites P(c) once P V(c) has read it
+                    if (c + 2 < nb) {
+                        if (!__all_sync(0xffffffffu, k_here)) warp_wait(ok, slot_full + 8 * ks, kph);
+                        issue_s(sb, ks);
+                    }
+                }
                 vs += c + 2 < nb ? 2 : 1;
                 if (vs >= SLOTS) {
                     vs -= SLOTS;
@@ -427,9 +449,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             auto read = [&]() {  // S is free for block c + 2
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_empty + 8 * group);
+                if constexpr (!S::kPTmem) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty + 8 * group);
+                }
             };
             float mx = -INFINITY;
 #pragma unroll 1
@@ -494,11 +518,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sum[(2 * i + 1) & 3] += __uint_as_float(w[i] & 0xffff0000u);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (h == 0 && c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);  // the buffer's last reader
-                unsigned char* prow = sm + S::kOffP + group * S::kPBytes + h * (kRows * 128) + r * 128;
+                if constexpr (S::kPTmem) {
+                    tmem_st_32x32b_x32(tmem_s + lane_off + kKeys * group, w);
+                    tmem_st_wait();
+                    tc_fence_before();
+                } else {
+                    if (h == 0 && c >= 2) wait_b(ok, pv_done + 8 * group, ((c - 2) >> 1) & 1);  // the buffer's last reader
+                    unsigned char* prow = sm + S::kOffP + group * S::kPBytes + h * (kRows * 128) + r * 128;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    *reinterpret_cast<uint4*>(prow + ((i ^ (r & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(prow + ((i ^ (r & 7)) << 4)) =
+                            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
             }
             if (key0 < s.lo || key0 + kKeys > s.hi) {
                 // V rows that no row of the tile sees; the block's V has its place in the ring to
@@ -513,7 +544,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     *reinterpret_cast<uint4*>(vt + (ch >> 3) * (kKeys * 128) + key * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
             }
-            fence_proxy_async();  // generic-proxy writes -> the MMA's async-proxy reads
+            if (!S::kPTmem || key0 < s.lo || key0 + kKeys > s.hi)
+                fence_proxy_async();  // generic-proxy writes -> the MMA's async-proxy reads
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + 8 * group);
         }
@@ -525,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int last = nb > 0 ? (nb - 1) & 1 : 0;
         if (group != last) {
-            s_sum[r] = l;  // where P was: every product is done
+            s_sum[r] = l;  // at the end of the ring: every product is done
             s_ref[r] = m;  // what it handed on last, if anything
             hand_on(9 + quad);
         } else {
@@ -543,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // Through the ring, whose copies and products are done, so that a warp writes whole
                 // rows: stored from the registers, a row a lane, they took three times as long.
                 constexpr int kPitch = HD * 4 + 16;  // lanes' rows start in different banks
-                static_assert(kRows * kPitch <= S::kOffP, "the output fits where the ring was");
+                static_assert(kRows * kPitch <= S::kOffSum, "the output fits where the ring was");
 #pragma unroll 1
                 for (int col = group * (HD / 2); col < (group + 1) * (HD / 2); col += 32) {
                     uint32_t o[32];

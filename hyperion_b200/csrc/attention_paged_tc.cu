@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const uint32_t tmem = __reduce_max_sync(0xffffffffu, *tmem_slot);
     const uint32_t tmem_s = tmem, tmem_o = tmem + 2 * kKeys, tmem_q = tmem_o + HD;
 
     int pmin = INT_MAX, pmax = -1;
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (per_request) so = segment<kKeys>(p.table + static_cast<size_t>(req) * p.max_blocks, p.prefix_len, own, pmin, pmax, p.window);
     const int all = sp.blocks + so.blocks;
     const int c0 = static_cast<int>(static_cast<long long>(all) * split / pl.tc_splits);
-    const int nb = __shfl_sync(0xffffffffu, static_cast<int>(static_cast<long long>(all) * (split + 1) / pl.tc_splits) - c0, 0);
+    const int nb = __reduce_max_sync(0xffffffffu, static_cast<int>(static_cast<long long>(all) * (split + 1) / pl.tc_splits) - c0);
     // the segment and first key of this part's block c
     auto block = [&](int c, int& key0) -> const Segment& {
         const int b = c0 + c;

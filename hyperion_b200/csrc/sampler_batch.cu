@@ -25,8 +25,8 @@
 // fp32 logits (sample_radix_kernel): the slice is held in shared memory, and the cut of
 // top-k / top-p is found by radix selection on an order-preserving 32-bit key, 11 bits a level:
 // each CTA fills a histogram of counts and weights (three 16-bit limbs, so that the shared
-// atomics stay native 32-bit ones), the cluster's first CTA adds the histograms up over
-// distributed shared memory and finds the bin in which the cut lies.
+// atomics stay native 32-bit ones), the bins that are not empty are added up in the cluster's
+// first CTA over distributed shared memory, which finds the bin in which the cut lies.
 #include "kernels.h"
 #include "tma.cuh"
 
@@ -53,6 +53,11 @@ struct Hist {
     uint32_t cnt[kBins], l0[kBins], l1[kBins], l2[kBins];
 };
 
+struct Merged {  // of all slices, in the cluster's first CTA
+    u64 mass[kBins];
+    uint32_t cnt[kBins];
+};
+
 struct Cut {       // where a level's cut lies
     uint32_t bin;
     uint32_t cnt;  // tokens above the bin
@@ -63,7 +68,8 @@ struct Cut {       // where a level's cut lies
 
 struct Share {  // read by the other CTAs of the cluster
     u64 best;       // (key of the maximum, ~index)
-    Cut cut;
+    Cut cut, got;   // found by the first CTA; as it sent it
+    uint32_t single;  // the only key left in the bin
     u64 sum;        // kept weight above the cut key
     uint32_t cnt;   // kept tokens above it
     uint32_t ties;  // tokens equal to it
@@ -97,15 +103,6 @@ __device__ __forceinline__ u64 cl_ld64(uint32_t a) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ uint4 cl_ld128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(a)
-                 : "memory");
-    return v;
-}
-
 // NaN -> -inf, -0 -> +0.
 __device__ __forceinline__ float canon(float x) { return x != x ? -INFINITY : x + 0.0f; }
 // Order-preserving key.
@@ -194,7 +191,8 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
     extern __shared__ __align__(16) unsigned char dyn[];
     __shared__ Share sh;
     Hist& h = *reinterpret_cast<Hist*>(dyn);
-    float* buf = reinterpret_cast<float*>(dyn + sizeof(Hist));
+    Merged& merged = *reinterpret_cast<Merged*>(dyn + sizeof(Hist));
+    float* buf = reinterpret_cast<float*>(dyn + sizeof(Hist) + sizeof(Merged));
     uint32_t nc;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nc));
     const uint32_t rank = cl_rank();
@@ -208,6 +206,11 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
     float tp = p.top_p ? p.top_p[row] : 0.f, mp = p.min_p ? p.min_p[row] : 0.f;
     const bool use_k = k > 0 && k < p.vocab, use_p = tp > 0.f && tp < 1.f, use_m = mp > 0.f;
     if (tid < 32) Weight::fill(sh.table);
+    if (rank == 0)
+        for (int i = tid; i < kBins; i += kThreads) {
+            merged.cnt[i] = 0;
+            merged.mass[i] = 0;
+        }
 
     // ---- the slice into shared memory, its maximum (first index)
     u64 best = 0;
@@ -250,7 +253,9 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
         sh.best = b;
     }
     cl_sync();
-    for (uint32_t r = 0; r < nc; ++r) best = max(best, cl_ld64(cl_map(&sh.best, r)));
+    best = lane < static_cast<int>(nc) ? cl_ld64(cl_map(&sh.best, lane)) : 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     const uint32_t arg = ~static_cast<uint32_t>(best);
     const float M = value_of(static_cast<uint32_t>(best >> 32));
     const float* x = resident ? buf : gx;
@@ -273,17 +278,29 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
         uint32_t above = 0;
         u64 mass_above = 0, target = 0;
         uint32_t in_bin = 0;
-        constexpr int LEVELS = 3;
 #pragma unroll 1
-        for (int level = 0; level < LEVELS; ++level) {
+        for (int level = 0; level < 3; ++level) {
             const int shift = level == 0 ? 21 : (level == 1 ? 10 : 0);
             const uint32_t width = level == 2 ? 10 : 11;
+            auto outside = [&](uint32_t key) { return level && (key >> (shift + width)) != (cut_key >> (shift + width)); };
+            if (level == 2 && in_bin == 1) {
+                // one token is left, as with 22 bits known there mostly is: whoever holds it says which
+                for (int i = tid; i < n; i += kThreads) {
+                    const uint32_t key = key_of(canon(x[i]));
+                    if (!outside(key))
+                        for (uint32_t r = 0; r < nc; ++r)
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cl_map(&sh.single, r)), "r"(key) : "memory");
+                }
+                cl_sync();
+                cut_key = sh.single;
+                break;
+            }
             for (int i = tid; i < 4 * kBins; i += kThreads) (&h.cnt[0])[i] = 0;
             __syncthreads();
             for (int i = tid; i < n; i += kThreads) {
                 const float xi = canon(x[i]);
                 const uint32_t key = key_of(xi);
-                if (level && (key >> (shift + width)) != (cut_key >> (shift + width))) continue;
+                if (outside(key)) continue;
                 const uint32_t bin = (key >> shift) & ((1u << width) - 1);
                 atomicAdd(&h.cnt[bin], 1u);
                 if (use_p) {
@@ -295,23 +312,27 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
                     }
                 }
             }
+            __syncthreads();
+            // the few hundred bins that are not empty go to the first CTA
+            const uint32_t to_cnt = cl_map(merged.cnt, 0), to_mass = cl_map(merged.mass, 0);
+            for (int i = tid; i < kBins; i += kThreads) {
+                const uint32_t cn = h.cnt[i];
+                if (!cn) continue;
+                asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(to_cnt + 4 * i), "r"(cn) : "memory");
+                const u64 m = h.l0[i] + (static_cast<u64>(h.l1[i]) << 16) + (static_cast<u64>(h.l2[i]) << 32);
+                if (m) asm volatile("red.shared::cluster.add.u64 [%0], %1;" ::"r"(to_mass + 8 * i), "l"(m) : "memory");
+            }
             cl_sync();
             if (rank == 0) {
                 // thread t takes bins from the top: 2047 - 4t - i
-                uint32_t bc[4] = {0, 0, 0, 0};
-                u64 bm[4] = {0, 0, 0, 0};
-                const int b0 = kBins - 4 - 4 * tid;
-                for (uint32_t r = 0; r < nc; ++r) {
-                    const uint4 a = cl_ld128(cl_map(&h.cnt[b0], r));
-                    const uint4 m0 = cl_ld128(cl_map(&h.l0[b0], r)), m1 = cl_ld128(cl_map(&h.l1[b0], r)),
-                                m2 = cl_ld128(cl_map(&h.l2[b0], r));
-                    const uint32_t av[4] = {a.w, a.z, a.y, a.x}, v0[4] = {m0.w, m0.z, m0.y, m0.x},
-                                   v1[4] = {m1.w, m1.z, m1.y, m1.x}, v2[4] = {m2.w, m2.z, m2.y, m2.x};
+                uint32_t bc[4];
+                u64 bm[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        bc[i] += av[i];
-                        bm[i] += v0[i] + (static_cast<u64>(v1[i]) << 16) + (static_cast<u64>(v2[i]) << 32);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    bc[i] = merged.cnt[kBins - 1 - 4 * tid - i];
+                    bm[i] = merged.mass[kBins - 1 - 4 * tid - i];
+                    merged.cnt[kBins - 1 - 4 * tid - i] = 0;  // for the next level
+                    merged.mass[kBins - 1 - 4 * tid - i] = 0;
                 }
                 uint32_t ct;
                 u64 mt;
@@ -330,15 +351,23 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
                     cum += bc[i];
                     cmass += bm[i];
                 }
+                __syncthreads();
+                if (tid < static_cast<int>(nc)) {
+                    const uint32_t at = cl_map(&sh.got, tid);
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + static_cast<uint32_t>(offsetof(Cut, bin))), "r"(sh.cut.bin) : "memory");
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + static_cast<uint32_t>(offsetof(Cut, cnt))), "r"(sh.cut.cnt) : "memory");
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + static_cast<uint32_t>(offsetof(Cut, in_bin))), "r"(sh.cut.in_bin) : "memory");
+                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at + static_cast<uint32_t>(offsetof(Cut, mass))), "l"(sh.cut.mass) : "memory");
+                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at + static_cast<uint32_t>(offsetof(Cut, total))), "l"(sh.cut.total) : "memory");
+                }
             }
             cl_sync();
-            const uint32_t a = cl_map(&sh.cut, 0);
-            cut_key |= cl_ld32(a + offsetof(Cut, bin)) << shift;
-            above = cl_ld32(a + offsetof(Cut, cnt));
-            in_bin = cl_ld32(a + offsetof(Cut, in_bin));
-            mass_above = cl_ld64(a + offsetof(Cut, mass));
-            target = cl_ld64(a + offsetof(Cut, total));
-            // the first CTA's next write of the cut lies behind the next level's first cluster barrier
+            cut_key |= sh.got.bin << shift;
+            above = sh.got.cnt;
+            in_bin = sh.got.in_bin;
+            mass_above = sh.got.mass;
+            target = sh.got.total;
+            // the first CTA's next write of it lies behind the next level's first cluster barrier
         }
         // all tokens of the last bin are equal: as many of them as the cut needs
         uint32_t take = in_bin;
@@ -1088,8 +1117,8 @@ void launch_f32(const SampleBatchParams& p, cudaStream_t stream) {
     while (nc < kMaxCluster && p.rows * nc * 2 <= num_sms() && p.vocab / nc >= 4096) nc *= 2;
     const int slice = ((p.vocab + nc - 1) / nc + 7) & ~7;
     const int resident = slice <= most ? 1 : 0;  // above 2^18 logits the slice stays in L2
-    allow_smem(reinterpret_cast<const void*>(sample_radix_kernel), sizeof(Hist) + kSliceBytes + 16);
-    launch_cluster(sample_radix_kernel, p.rows, nc, kThreads, sizeof(Hist) + (resident ? slice * 4 : 0), stream, p, slice, resident);
+    allow_smem(reinterpret_cast<const void*>(sample_radix_kernel), sizeof(Hist) + sizeof(Merged) + kSliceBytes);
+    launch_cluster(sample_radix_kernel, p.rows, nc, kThreads, sizeof(Hist) + sizeof(Merged) + (resident ? slice * 4 : 0), stream, p, slice, resident);
 }
 
 }  // namespace

@@ -104,6 +104,17 @@ Way way_of(const Sizes& z, int window) {
     return together < apart ? Way::kTogether : Way::kApart;
 }
 
+// Whether the kernel's 32-bit numbers of slices could overflow (some room left for tiles that begin
+// inside a slice). Requests' rows are disjoint, so that the tiles are at most those of all rows and
+// one more each.
+bool too_many_slices(const Sizes& z, const SharedPlan& s) {
+    if (s.shares == 0) return false;
+    auto slices = [](long long keys) { return (keys + kSlice - 1) / kSlice; };
+    const long long tiles = std::min(static_cast<long long>(z.n_req) * s.tiles_o, z.all_rows / kTileRows + z.n_req);
+    const double all = static_cast<double>(tiles) * static_cast<double>(slices(z.max_own) + (s.o_prefix ? slices(z.prefix_len) : 0));
+    return all + static_cast<double>(slices(z.prefix_len)) >= 2147483648.;
+}
+
 SharedPlan plan_of(const Sizes& z, Way way, int window) {
     SharedPlan s;
     if (way == Way::kPerRequest) {
@@ -284,8 +295,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         // which shares have a piece of a unit: for the merge, every unit by one CTA
         auto pieces = [&](unsigned a, int n) {
             if (total == 0 || n == 0) return make_int2(0, 0);
-            const unsigned w0 = static_cast<unsigned>((static_cast<uint64_t>(a + 1) * shares - 1) / total);
-            const unsigned w1 = static_cast<unsigned>((static_cast<uint64_t>(a + n) * shares - 1) / total);
+            auto share_of = [&](uint64_t end) { return min(static_cast<unsigned>((end * shares - 1) / total), shares - 1); };
+            const unsigned w0 = share_of(static_cast<uint64_t>(a) + 1), w1 = max(w0, share_of(static_cast<uint64_t>(a) + n));
             return make_int2(static_cast<int>(w0), static_cast<int>(w1 - w0 + 1));
         };
         if (blockIdx.x == 0 && threadIdx.x == 0 && pl.prefix_unit) parts.unit[0] = pieces(0, prefix_slices);
@@ -329,10 +340,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             }
             req = lo;
             n = s_slices[req];
-            const int rel = r0 - s_start[req];
-            tile = rel / n;
+            const unsigned rel = r0 - s_start[req];
+            tile = min(static_cast<int>(rel / n), pl.tiles_o - 1);
             unit = pl.prefix_unit + req * pl.tiles_o + tile;
-            s0 = rel - tile * n;
+            s0 = static_cast<int>(rel % n);
         }
         mine = min(static_cast<int>(r1 - r0), n - s0);
         r0 += mine;
@@ -780,6 +791,7 @@ size_t shared_attn_scratch_bytes(int T, int n_req, int max_q, int max_own, int p
 void launch_shared_attn(const SharedAttnParams& p, cudaStream_t stream) {
     const Sizes z(p.T, p.n_req, p.max_q, p.max_own, p.prefix_len, p.n_heads, p.n_kv, p.hd);
     const SharedPlan pl = plan_of(z, way_of(z, p.window), p.window);
+    if (too_many_slices(z, pl)) throw ArgError("sdpa_shared_prefix: 2^31 or more steps of 16 keys");
     const Layout at(pl, p.T, p.n_req, p.n_heads, p.n_kv, p.hd);
     if (p.scratch_bytes < at.bytes + 512) throw ArgError("sdpa_shared_prefix: scratch too small");
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p.scratch) + 255) & ~static_cast<uintptr_t>(255));

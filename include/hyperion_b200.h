@@ -296,7 +296,9 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   after the last key that its rows see may hold anything (NaN included), those between
  *   must be finite.
  * n_req is 1..1024; head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; n_pages *
- * page_size < 2^31; q, the pools, out and scratch 16-byte aligned.
+ * page_size < 2^31; q, the pools, out and scratch 16-byte aligned, and neither out nor scratch
+ * overlaps anything else. A call is refused when its steps of 16 keys, by the bounds and for every
+ * 16 (row, head) pairs of a KV head, could be 2^31 or more.
  */
 size_t hyb_sdpa_shared_prefix_scratch_bytes(int32_t T, int32_t n_req, int32_t max_q, int32_t max_own,
                                             int32_t prefix_len, int32_t n_heads, int32_t n_kv, int32_t head_dim);

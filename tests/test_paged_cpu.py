@@ -61,6 +61,13 @@ def test_attn_refuses(built_lib, kw):
     assert _attn(built_lib, **kw) == hb.INVALID_ARGUMENT
 
 
+def test_attn_refuses_too_many_steps(built_lib):
+    # 1024 requests of one row each, their own keys of 2^25 tokens: 2^31 steps of 16 keys
+    kw = dict(T=1024, n_req=1024, max_q=1, plen=0, pt=None, nbytes=1 << 40)
+    assert _attn(built_lib, max_own=1 << 25, **kw) == hb.INVALID_ARGUMENT
+    assert "steps of 16 keys" in hb.last_error()
+
+
 @pytest.mark.parametrize("kw", [dict(hd=32), dict(hd=512), dict(page=8), dict(page=48), dict(page=512)])
 def test_attn_unsupported(built_lib, kw):
     assert _attn(built_lib, **kw) == hb.UNSUPPORTED

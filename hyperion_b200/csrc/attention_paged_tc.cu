@@ -28,10 +28,15 @@
 //
 // Measured on a B200. head_dim 256, 16 query and 8 KV heads, 8 requests of 200 to 300 rows on a
 // prefix of 8192 and up to 600 own tokens: 324 us, 846 TFLOP/s, half of what a large dense
-// product reaches; a 64-key block takes some 2100 cycles, of which S alone takes 1150 (its
-// products are 64 columns wide, and Q's TMEM operand is read anew for each). The products bound it:
-// a copy of the kernel without the exponentials, and one without the copies of K and V, took as
-// long. head_dim 128, 32 query and 16 KV heads, 64 rows on a 16384-token prefix: 35 us for 134 MB of
+// product reaches. A 64-key block takes some 2100 cycles, its products alone 1270 of them (a
+// product of 128 x 64 x 16 takes 47, of 128 x 128 x 16 64, of 128 x 256 x 16 128); the rest is the chain
+// softmax(c) -> P V(c) -> S(c + 2) of the two blocks in flight, and the waits and commits of the issuing
+// warp between its products (a wait on a complete barrier 109 cycles, a commit 40). Copies of the
+// kernel without the exponentials, and without the copies of K and V, took as long. Tried: S of
+// 128 columns with the queries in shared memory (310 us, but few rows with a window 32 -> 35 us),
+// that with S and P V issued by a warp each or with the scores held in registers (the same), and
+// with loops of 32 keys (327 us).
+// head_dim 128, 32 query and 16 KV heads, 64 rows on a 16384-token prefix: 35 us for 134 MB of
 // keys and values and 17.2 GFLOP (3.8 TB/s, 490 TFLOP/s).
 #include "attention_paged.cuh"
 #include "tcgen05.cuh"

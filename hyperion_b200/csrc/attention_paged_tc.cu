@@ -139,13 +139,6 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // Hand-over between warp w of one softmax group and warp w of the other.
 __device__ __forceinline__ void hand_on(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ void take_over(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-// 32 bytes to global memory (a whole sector).
-__device__ __forceinline__ void st_v8(float* p, const uint32_t* r) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-
 // The keys of one segment (prefix or own) that a tile of rows sees: [lo, hi), in blocks from `first` on.
 struct Segment {
     const int* table;
@@ -631,8 +624,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = shared_pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-                    st_v8(reinterpret_cast<float*>(dst + col / 2), w);
-                    st_v8(reinterpret_cast<float*>(dst + col / 2 + 8), w + 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)  // 16 bytes at a time: rows start at no wider boundary
+                        *reinterpret_cast<uint4*>(dst + col / 2 + 4 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 }
             }
         }

@@ -64,6 +64,9 @@ __device__ __forceinline__ long long block_scan_ll(long long v, long long* total
     return before + inc - v;
 }
 
+// Pages that hold c >= 0 tokens; c + P - 1 may pass 2^31.
+__device__ __forceinline__ int pages_of(int c, int P) { return c == 0 ? 0 : (c - 1) / P + 1; }
+
 // The last index i in [0, n) with a[i] <= v (a ascending, a[0] <= v).
 __device__ __forceinline__ int last_le(const int* a, int n, int v) {
     int lo = 0, hi = n;  // a[lo] <= v, a[hi] > v or hi == n
@@ -149,15 +152,16 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPla
     __syncthreads();
 
     // ---- the pages taken, entered in their requests' tables
-    const int nthreads = gridDim.x * kPlanThreads, me = blockIdx.x * kPlanThreads + threadIdx.x;
+    const unsigned nthreads = gridDim.x * kPlanThreads, me = blockIdx.x * kPlanThreads + threadIdx.x;
     for (long long j = me; j < pages; j += nthreads) {
         const int b = last_le(s_page, n, static_cast<int>(j));
-        const int held = (s_cached[b] + P - 1) / P;
+        const int held = pages_of(s_cached[b], P);
         p.table[static_cast<size_t>(b) * p.max_blocks + held + (j - s_page[b])] = p.free_pages[j];
     }
     // ---- rows; a row's page is an old entry of the table (which nobody writes here) or an
     // entry of the free list
-    for (int r = me; r < p.max_rows; r += nthreads) {
+    for (unsigned at_row = me; at_row < static_cast<unsigned>(p.max_rows); at_row += nthreads) {  // signed, the last step could pass 2^31
+        const int r = static_cast<int>(at_row);
         int req = -1, pos = -1, slot = -1;
         if (r < n_rows) {
             req = last_le(s_row, n, r);
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPla
             pos = static_cast<int>(min(p.pos0 + at, static_cast<long long>(INT_MAX)));
             if (sc >= 0) {
                 const int local = static_cast<int>(at);  // inside the table
-                const int blk = local / P, held = (c + P - 1) / P;
+                const int blk = local / P, held = pages_of(c, P);
                 const int page = blk < held ? p.table[static_cast<size_t>(req) * p.max_blocks + blk]
                                             : p.free_pages[s_page[req] + blk - held];
                 if (page >= 0 && page < p.n_pages) slot = page * P + local % P;
@@ -298,7 +302,7 @@ void launch_paged_plan(const PagedPlanParams& p, cudaStream_t stream) {
     const size_t smem = static_cast<size_t>(p.n_req) * 3 * sizeof(int);
     allow_smem(reinterpret_cast<const void*>(paged_plan_kernel), kMaxPlanRequests * 3 * sizeof(int));
     // one row a thread until every SM has a CTA
-    const int blocks = std::max(1, std::min((p.max_rows + kPlanThreads - 1) / kPlanThreads, num_sms()));
+    const int blocks = std::max(1, std::min((p.max_rows - 1) / kPlanThreads + 1, num_sms()));
     paged_plan_kernel<<<blocks, kPlanThreads, smem, stream>>>(p);
     HYB_LAUNCH_CHECK("paged_plan_kernel");
 }

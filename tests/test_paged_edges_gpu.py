@@ -2,12 +2,42 @@
 
 Roundings as in test_paged_gpu.py: bf16 half a step is 2^-8 of the value, fp32 2^-24.
 """
+import numpy as np
 import pytest
 
 from tests.conftest import has_gpu
-from tests.test_paged_gpu import Batch, _no_timeouts  # noqa: F401
+from tests.test_paged_gpu import Batch, _no_timeouts, run_plan  # noqa: F401
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not has_gpu(), reason="no CUDA device")]
+
+
+# ---------------------------------------------------------------------------------- plan
+@pytest.mark.parametrize("page,cached,new", [(2 ** 31 - 1, [2 ** 30 + 5, 2, 2 ** 31 - 4, 0], [3, 1, 3, 2]), (2 ** 30 + 1, [2 ** 30 - 1, 0], [2, 4]),
+                                             (1000, [2147482990, 2147482000, 0], [5, 3, 1])])
+def test_plan_lengths_whose_rounding_up_passes_32_bits(built_lib, page, cached, new):
+    width = (2 ** 31 - 1) // page
+    n = len(cached)
+    table = np.zeros((n, width), np.int64)
+    for b in range(n):
+        table[b, -1] = b % width  # pages of the pool: 0 .. width - 1
+    run_plan(np.array(cached), np.array(new), np.arange(n) % width, table, width, page, sum(new) + 2)
+
+
+def test_plan_most_rows(built_lib):
+    """2^31 - 1 rows: every one behind the last is -1, up to the end of each array."""
+    import torch
+    from hyperion_b200 import ops
+    rows = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    plan = ops.paged_plan(i32(0, 7), i32(3, 2), i32(5, 6, 7), torch.zeros(2, 4, dtype=torch.int32, device="cuda"), 8, 16, rows)
+    assert plan.row_start.tolist() == [0, 3, 5] and plan.status.tolist() == [1, 5, 0, 0]
+    assert plan.row_pos[:5].tolist() == [0, 1, 2, 7, 8] and plan.slot_map[:5].tolist() == [80, 81, 82, 7, 8]
+    for x in (plan.row_req, plan.row_pos, plan.slot_map):
+        assert all(int(x[i:i + 2 ** 29].max()) == -1 == int(x[i:i + 2 ** 29].min()) for i in range(5, rows, 2 ** 29))
+    del plan, x
+    torch.cuda.empty_cache()
 
 
 # ----------------------------------------------------------------------------- attention

@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 namespace hyb {
@@ -35,6 +36,24 @@ HypStatus run(Fn&& fn) noexcept {
 }
 
 inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
+// Whether an output overlaps an input or another output (empty and null ones overlap nothing).
+struct Span {
+    const void* p;
+    size_t bytes;
+    bool meets(const Span& o) const {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
+        return p && o.p && a < b + o.bytes && b < a + bytes;
+    }
+};
+bool outputs_overlap(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+    for (const Span* o = outputs.begin(); o != outputs.end(); ++o) {
+        for (const Span* q = outputs.begin(); q != o; ++q)
+            if (o->meets(*q)) return true;
+        for (const Span& i : inputs)
+            if (o->meets(i)) return true;
+    }
+    return false;
+}
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
@@ -410,6 +429,11 @@ HypStatus hyb_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, in
         return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: bad shape");
     if (static_cast<int64_t>(n_pages) * page_size > INT32_MAX || static_cast<int64_t>(max_blocks) * page_size + pos0 > INT32_MAX)
         return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: slots and positions must stay below 2^31");
+    const size_t per_req = sizeof(int32_t) * n_req, per_row = sizeof(int32_t) * max_rows;
+    if (outputs_overlap({{block_table, per_req * max_blocks}, {row_start, per_req + sizeof(int32_t)}, {row_req, per_row}, {row_pos, per_row},
+                         {slot_map, per_row}, {total_lens, per_req}, {status, 4 * sizeof(int32_t)}},
+                        {{cached_lens, per_req}, {new_lens, per_req}, {free_pages, sizeof(int32_t) * n_free}}))
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "paged_plan: an output overlaps an input or another output");
     return run([&] {
         hyb::PagedPlanParams p;
         p.cached = cached_lens;

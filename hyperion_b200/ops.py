@@ -227,7 +227,8 @@ class PagedPlan:
 
 def paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages: int, page_size: int, max_rows: int, pos0=0,
                plan: PagedPlan | None = None, stream=None) -> PagedPlan:
-    """Block tables (in place) and the row tables of a step from the requests' lengths."""
+    """Block tables (in place) and the row tables of a step from the requests' lengths. The lengths may be
+    another plan's total_lens, not those of the `plan` that is written."""
     dev, n = _device(cached_lens), cached_lens.numel()
     if block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("block_table is [n_req, max_blocks], free_pages [n_free]")

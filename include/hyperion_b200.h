@@ -253,7 +253,9 @@ HypStatus hyb_sample_logits(const void* logits, int32_t n, const HypSamplingConf
  *   negative, its tokens do not fit max_blocks, its rows do not fit max_rows, or the free list
  *   is used up: it takes no page, total_lens stays cached (0 if that is negative), and its rows
  *   (none if a length is negative) get slot -1. A later request that needs no page still runs.
- * n_req is 1..8192; n_pages * page_size and pos0 + max_blocks * page_size are below 2^31.
+ * n_req is 1..8192; n_pages * page_size and pos0 + max_blocks * page_size are below 2^31. No output
+ * (block_table among them) may overlap an input or another output: to step from total_lens, copy it
+ * to cached_lens or let two sets of outputs take turns.
  */
 HypStatus hyb_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int32_t n_req, int32_t page_size,
                          int32_t n_pages, const int32_t* free_pages, int32_t n_free, int32_t* block_table,

@@ -40,6 +40,27 @@ def test_plan_most_rows(built_lib):
     torch.cuda.empty_cache()
 
 
+def test_plan_stepped_from_its_own_lengths(built_lib):
+    """total_lens is the next step's cached_lens: of the same plan refused, of two in turn right."""
+    import torch
+    import hyperion_b200 as hb
+    from hyperion_b200 import ops
+    n, page, rows = 1000, 16, 3000
+    rng = np.random.default_rng(1)
+    table = torch.zeros(n, 8, dtype=torch.int32, device="cuda")
+    free = torch.arange(4000, dtype=torch.int32, device="cuda")
+    lens, done = torch.zeros(n, dtype=torch.int32, device="cuda"), np.zeros(n, np.int64)
+    plans = [ops.PagedPlan(n, rows), ops.PagedPlan(n, rows)]
+    for i in range(6):
+        new = rng.integers(0, 4, n)
+        plan = ops.paged_plan(lens, torch.tensor(new, dtype=torch.int32, device="cuda"), free, table, 4000, page, rows, plan=plans[i % 2])
+        done += new
+        assert plan.total_lens.tolist() == done.tolist() and plan.status[1:].tolist() == [int(new.sum()), 0, 0]
+        free, lens = free[int(plan.status[0]):].contiguous(), plan.total_lens
+        with pytest.raises(hb.HypError, match="overlap"):
+            ops.paged_plan(lens, torch.ones(n, dtype=torch.int32, device="cuda"), free, table, 4000, page, rows, plan=plan)
+
+
 # ----------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("B,q,prefix", [(2, 150, 300), (2, 1, 30), (40, 1, 300), (4, 1, 300)])

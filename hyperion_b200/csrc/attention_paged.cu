@@ -415,9 +415,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         const int key = a ? ka.first + s * kSlice : kb.first + (s - ka.slices) * kSlice;
         if ((from > 0 || p.window > 0) && i < mine) pages = (a ? ka.table : kb.table)[key >> page_shift];
         const bool there = pages >= 0 && pages < p.n_pages;
-        if (i < mine && !there) bad = true;
+        const bool seen = i < mine && key < (a ? ka.hi : kb.hi);
+        if (seen && !there) bad = true;
         // slices without a visible key, and bad pages: a box past the pool, which reads as zeros
-        pages = i < mine && there && key < (a ? ka.hi : kb.hi) ? (pages << page_shift) + (key & in_page) : p.n_pages << page_shift;
+        pages = seen && there ? (pages << page_shift) + (key & in_page) : p.n_pages << page_shift;
     };
     int f_slot = slot;
     auto fetch = [&](int j) {  // K (even) or V (odd) of this warp's slice j / 2

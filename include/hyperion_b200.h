@@ -292,8 +292,9 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   max_q and max_own are host bounds on a request's rows and own keys: they size the launch
  *   and the scratch (hyb_sdpa_shared_prefix_scratch_bytes with the same values; contents do
  *   not matter before or after). Rows at or past max_q of a request, and rows of a request
- *   with more than max_own or max_blocks * page_size keys, become NaN; so do rows some of
- *   whose tile of rows read a page outside [0, n_pages). A negative own_lens counts as 0.
+ *   with more than max_own or max_blocks * page_size keys, become NaN; so do rows with a key to
+ *   see, in their tile of rows, on a page outside [0, n_pages). Entries of pages on which no row sees
+ *   a key may be anything. A negative own_lens counts as 0.
  *   A request's rows are taken to stand at neighbouring positions: slots before the first and
  *   after the last key that its rows see may hold anything (NaN included), those between
  *   must be finite.

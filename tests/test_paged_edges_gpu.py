@@ -77,3 +77,29 @@ def test_attn_output_on_any_16_byte_boundary(built_lib, hd, B, q, prefix):
         b.call(out=out)
         assert torch.equal(out, want)
         assert (flat[:off] == 7.0).all() and (flat[off + n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("B,q,prefix,own", [(3, 1, 0, 80), (3, 1, 100, 300), (40, 1, 100, 300), (2, 70, 100, 300)])
+def test_attn_pages_that_no_row_sees(built_lib, hd, B, q, prefix, own):
+    """Rows that stand before their request's last keys: the pages behind them are not looked at."""
+    import torch
+    start = prefix + own - q - 33  # two pages and more end unseen
+    b = Batch(4, 2, hd, 16, prefix, [own] * B, [q] * B, seed=hd + B, positions=np.tile(start + np.arange(q), B))
+    for page in (-1, 10 ** 6):
+        c = b.table.copy()
+        b.table[:, (own - 1) // 16] = page
+        got = b.call()
+        b.table = c
+        b.check(got, rows=list(range(min(b.T, 12))) + [b.T - 1])
+        assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("prefix", [300, 700])
+def test_attn_prefix_pages_that_no_row_sees(built_lib, prefix):
+    b = Batch(4, 2, 64, 16, prefix, [3, 2], [1, 1], seed=prefix, positions=[100, 90])
+    tab = b.ptab.copy()
+    b.ptab[7:] = -1
+    got = b.call()
+    b.ptab = tab
+    b.check(got)

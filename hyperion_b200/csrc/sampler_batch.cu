@@ -167,6 +167,18 @@ struct Weight {
     }
 };
 
+// The least logit that min-p keeps: exp((x - M) / T) >= min_p where x >= M + T ln(min_p). Compared
+// in logits and not in weights, whose roundings (2^-27, and 2^-44 of the largest) would put close
+// logits on the wrong side and lose all settings below 2^-45. Formed in double, with exp taken as
+// rounded to it (half a step below 1 is 2^-54), and rounded up, so that a float is at least this
+// one just when it is at least the double. min_p above 1 counts as 1.
+__device__ __forceinline__ float min_p_floor(float M, float temperature, float min_p) {
+    if (M == INFINITY) return M;
+    const double lg = log(static_cast<double>(fminf(min_p, 1.f))) - 5.5511151231257827e-17;
+    const float least = __double2float_ru(static_cast<double>(M) + static_cast<double>(temperature) * lg);
+    return fmaxf(least, -3.402823466e38f);  // never -inf, whose weight is 0
+}
+
 // Inclusive block scan in thread order; *total is the block's sum.
 template <typename V>
 __device__ __forceinline__ V block_incl(V v, V* red, V* total) {
@@ -383,8 +395,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
     }
 
     // ---- kept weights: warp w of the CTA owns a contiguous run of its slice
-    const double mpd = static_cast<double>(fminf(mp, 1.f)) * 17592186044416.0;  // min_p in units of 2^-44
-    auto passes = [&](u64 w) { return !use_m || static_cast<double>(w) >= mpd; };
+    const float least = use_m ? min_p_floor(M, temp, mp) : -INFINITY;
     const int run = ((slice + kWarpsS - 1) / kWarpsS + 31) & ~31;
     {
         const int from = warp * run, to = min(n, from + run);
@@ -397,9 +408,8 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
                 ties += key == cut_key;
                 continue;
             }
-            const u64 w = weight(xi);
-            if (passes(w)) {
-                sum += w;
+            if (xi >= least) {
+                sum += weight(xi);
                 ++cnt;
             }
         }
@@ -430,7 +440,7 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
     }
     cl_sync();
     u64 tie_w = cut ? weight(value_of(cut_key)) : 0;
-    if (cut && !passes(tie_w)) {
+    if (cut && value_of(cut_key) < least) {
         tie_w = 0;
         ties_kept = 0;
     }
@@ -477,9 +487,8 @@ __global__ void __launch_bounds__(kThreads) sample_radix_kernel(const SampleBatc
         const float xi = canon(x[i]);
         const uint32_t key = key_of(xi);
         tie = cut && key == cut_key;
-        if (cut && key <= cut_key) return 0;
-        const u64 w = weight(xi);
-        return passes(w) ? w : 0;
+        if ((cut && key <= cut_key) || xi < least) return 0;
+        return weight(xi);
     };
     for (int i = i0; i < i1; ++i) {
         bool tie;
@@ -844,29 +853,12 @@ __global__ void __launch_bounds__(kHThreads, 1) sample_hist_kernel(const SampleB
             }
             __syncthreads();
             if (use_m) {
-                // min-p: the kept tokens with w >= min_p; where the cut's own weight passes nothing changes
-                const double mpd = static_cast<double>(fminf(mp, 1.f)) * 17592186044416.0;
-                const uint32_t kc = sh.cut;
-                const bool cut_passes = kc < 65536u && static_cast<double>(weight(value_at(kc))) >= mpd;
-                if (!cut_passes) {
-                    // weights fall along the places, so the passing places are a prefix, which ends before the
-                    // cut: near M + T ln(min_p), found there by 32 places at a time
-                    const float guess = M + temp * logf(fminf(mp, 1.f));
-                    int first = static_cast<int>(place_of(__bfloat16_as_ushort(f2bf(guess)))) - 16;
-                    uint32_t end = 0;
-                    for (int way = 0;;) {  // up or down, never back
-                        first = max(0, min(first, 65536 - 32));
-                        const uint32_t o = first + lane;
-                        const float x = is_nan_place(o) ? (o < 32768u ? INFINITY : -INFINITY) : value_at(o);
-                        const bool pass = x >= M || static_cast<double>(weight(x)) >= mpd;
-                        const int passing = __popc(__ballot_sync(0xffffffffu, pass));
-                        end = first + passing;
-                        if (passing == 32 && first < 65536 - 32 && way >= 0) way = 1;
-                        else if (passing == 0 && first > 0 && way <= 0) way = -1;
-                        else break;
-                        first += 32 * way;
-                    }
-                    end = min(end, kc);
+                // min-p: the places down to that of the least bf16 at or above the floor; where the cut
+                // lies among them nothing changes
+                const uint32_t f = __float_as_uint(min_p_floor(M, temp, mp) + 0.f);
+                uint32_t end = place_of((f & 0x80000000u ? f : f + 0xffffu) >> 16) + 1;
+                if (end == kPlaceNegZero) ++end;  // both zeros or none
+                if (sh.cut >= end) {
                     const uint32_t ge = end >> 5;
                     __syncthreads();
                     if (2 * tid <= ge && ge <= 2 * tid + 1) {

@@ -321,7 +321,8 @@ HypStatus hyb_sdpa_shared_prefix(const void* q, const void* k_pool, const void* 
  * min_p (off unless > 0), and u in [0, 1).
  *   Weights are w = exp((x - max x) / temperature), tokens ordered by logit descending, then
  *   index ascending. Each filter keeps a prefix of that order: the first top_k; the shortest
- *   whose weight reaches top_p of the whole row's; those with w >= min_p. The shortest of the
+ *   whose weight reaches top_p of the whole row's; those with w >= min_p (above 1 counts as 1; compared in
+ *   logits, x >= max x + temperature * ln(min_p), however small the weight). The shortest of the
  *   three is kept, and token is the first index, in index order, at which the running sum
  *   of the kept weights exceeds u times their sum. temperature <= 0 (or NaN) takes the
  *   first maximum. kept (may be null) is the number of tokens kept, prob (may be null) the

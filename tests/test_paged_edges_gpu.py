@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from tests.conftest import has_gpu
-from tests.test_paged_gpu import Batch, _no_timeouts, run_plan  # noqa: F401
+from tests.test_paged_gpu import Batch, _no_timeouts, run_plan, run_sample  # noqa: F401
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not has_gpu(), reason="no CUDA device")]
 
@@ -103,3 +103,44 @@ def test_attn_prefix_pages_that_no_row_sees(built_lib, prefix):
     got = b.call()
     b.ptab = tab
     b.check(got)
+
+
+# ------------------------------------------------------------------------------ sampling
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("min_p", [1e-12, 1e-14, 1e-20, 1e-37])
+def test_min_p_below_the_weights_resolution(built_lib, dtype, min_p):
+    """exp((x - M) / T) >= min_p down to where the weights of 44 bits are all zero."""
+    import torch
+    rng = np.random.default_rng(3)
+    x = np.stack([np.linspace(-130, 4, 5001), rng.permutation(np.linspace(-130, 4, 5001)), rng.standard_normal(5001) * 30,
+                  np.where(np.arange(5001) % 3, -np.inf, np.linspace(-100, 100, 5001))]).astype(np.float32)
+    run_sample(x, [0.2, 0.9, 0.5, 0.7], [1.0, 1.3, 0.7, 2.5], 0, 0.0, min_p, getattr(torch, dtype))
+    run_sample(x, [0.2, 0.9, 0.5, 0.7], [1.0, 1.3, 0.7, 2.5], [0, 4000, 30, 0], [0.9999, 0.0, 0.0, 0.5], min_p, getattr(torch, dtype))
+
+
+@pytest.mark.parametrize("min_p", [0.3, 0.5, 0.77, 0.9])
+def test_min_p_between_neighbouring_logits(built_lib, min_p):
+    """Thousands of neighbouring fp32 logits on both sides of M + T ln(min_p): the kept ones are those above it,
+    whatever the roundings of their weights."""
+    import torch
+    rng = np.random.default_rng(int(min_p * 100))
+    rows = []
+    for M in (0.0, 0.25, 1.0):
+        at = np.float32(M + np.log(np.float64(np.float32(min_p))))
+        near = (at.view(np.int32) + np.arange(-3000, 3000, dtype=np.int32)).view(np.float32)
+        rows.append(np.concatenate([rng.permutation(near), np.float32([M])]))
+    run_sample(np.stack(rows), [0.25, 0.5, 0.75], 1.0, 0, 0.0, min_p, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_min_p_around_zero_logits(built_lib, dtype):
+    """The least kept logit is a zero, of either sign."""
+    import torch
+    x = np.zeros((6, 300), np.float32)
+    x[:, ::2] = -0.0
+    x[:, 100:200] = -1e-3
+    x[1, 7] = x[4, 7] = np.log(4.0)
+    x[2:4, 150] = 1e-38
+    x[3, 151] = -1e-38
+    run_sample(x, [0.1, 0.2, 0.5, 0.6, 0.9, 0.99], [1.0, 1.0, 1e-3, 1e-3, 2.0, 1e-5], 0, 0.0, [1.0, 0.25, 1.0, 0.5, 0.5, 1.0],
+               getattr(torch, dtype))

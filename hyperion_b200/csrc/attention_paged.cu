@@ -134,6 +134,9 @@ SharedPlan plan_of(const Sizes& z, Way way, int window) {
     const long long prefix_slices = (z.prefix_len + kSlice - 1) / kSlice;
     const long long unit_slices = (z.max_own + kSlice - 1) / kSlice + (s.o_prefix ? prefix_slices : 0);
     if (unit_slices > 0) s.tiles_o = z.tiles_o;
+    const bool by_rows = static_cast<long long>(z.n_req) * s.tiles_o > z.all_rows / kTileRows + z.n_req;
+    s.unit_req = by_rows ? 1 : s.tiles_o;
+    s.unit_rows = by_rows ? z.n_heads / z.n_kv : 0;
     if (way == Way::kTogether && unit_slices > 0 && unit_slices <= kWarps * kMinSlices) {
         s.one_part = 1;
         return s;
@@ -302,9 +305,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             return make_int2(static_cast<int>(w0), static_cast<int>(w1 - w0 + 1));
         };
         if (blockIdx.x == 0 && threadIdx.x == 0 && pl.prefix_unit) parts.unit[0] = pieces(0, prefix_slices);
-        for (int i = blockIdx.x * kWarps * 32 + threadIdx.x; i < p.n_req * pl.tiles_o; i += gridDim.x * kWarps * 32) {
-            const int b = i / pl.tiles_o;
-            parts.unit[pl.prefix_unit + i] = pieces(s_start[b] + (i - b * pl.tiles_o) * s_slices[b], s_slices[b]);
+        if (pl.unit_rows == 0) {
+            for (int i = blockIdx.x * kWarps * 32 + threadIdx.x; i < p.n_req * pl.tiles_o; i += gridDim.x * kWarps * 32) {
+                const int b = i / pl.tiles_o;
+                parts.unit[pl.prefix_unit + i] = pieces(s_start[b] + (i - b * pl.tiles_o) * s_slices[b], s_slices[b]);
+            }
+        } else {
+            for (int b = blockIdx.x * kWarps + warp; b < p.n_req; b += gridDim.x * kWarps) {
+                const Request r = request_of(p, b);
+                const int tiles = min(pl.tiles_o, static_cast<int>((static_cast<long long>(r.n_tok) * G + kTileRows - 1) / kTileRows));
+                for (int i = lane; i < tiles; i += 32) parts.unit[pl.unit_of(b, r.t0, i)] = pieces(s_start[b] + i * s_slices[b], s_slices[b]);
+            }
         }
     }
 
@@ -313,11 +324,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll 1
     for (bool more = true; more;) {
     // ---- which unit, and which of its slices: i-th one s0 + i * stride
-    int req, tile, hk, s0, mine, unit;
+    int req, tile, hk, s0, mine;
     constexpr int stride = ONE ? kWarps : 1;
     if constexpr (ONE) {
         hk = blockIdx.x % p.n_kv;
-        unit = blockIdx.x / p.n_kv;
+        const int unit = blockIdx.x / p.n_kv;
         tile = unit % pl.tiles_o;
         req = unit / pl.tiles_o;
         s0 = warp;
@@ -328,7 +339,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         int n;
         hk = my_hk;
         if (r0 < prefix_slices) {
-            unit = 0;
             tile = 0;
             req = -1;
             n = prefix_slices;
@@ -344,7 +354,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             n = s_slices[req];
             const unsigned rel = r0 - s_start[req];
             tile = min(static_cast<int>(rel / n), pl.tiles_o - 1);
-            unit = pl.prefix_unit + req * pl.tiles_o + tile;
             s0 = static_cast<int>(rel % n);
         }
         mine = min(static_cast<int>(r1 - r0), n - s0);
@@ -561,6 +570,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         mA = mB = 0.f;
     }
     if constexpr (!ONE) {
+        const int unit = req < 0 ? 0 : pl.unit_of(req, t0, tile);
         const size_t place = (static_cast<size_t>(my_share + unit) * p.n_kv + hk) * kTileRows;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -651,6 +661,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParam
             first = __shfl_sync(0xffffffffu, v, more);
         }
         live = live && t >= begin && t < end && pos >= 0;
+        first = max(first, 0);
         if (live) {
             const int own = p.own_lens[req];
             broken = t - first >= p.max_q || own > p.max_own || own > static_cast<long long>(p.max_blocks) * p.page_size;
@@ -672,7 +683,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnParam
             m0 = t * G + g;
         }
         if (pl.tiles_o > 0) {
-            const int m = (t - first) * G + g, unit = pl.prefix_unit + req * pl.tiles_o + m / kTileRows;
+            const int m = (t - first) * G + g, unit = pl.unit_of(req, first, m / kTileRows);
             const int2 u = parts.unit[unit];
             a1 = u.x + unit;
             n1 = u.y;
@@ -743,7 +754,8 @@ struct Layout {
     size_t o, ml, po, pml, unit, bytes;
     Layout(const SharedPlan& s, int T, int n_req, int n_heads, int n_kv, int hd) {
         rows = s.direct() ? 0 : static_cast<long long>(T) * n_heads * s.tc_splits;
-        units = s.direct() ? 0 : s.prefix_unit + static_cast<long long>(n_req) * s.tiles_o;
+        units = s.direct() ? 0 : s.prefix_unit + (s.unit_rows > 0 ? static_cast<long long>(T) * (n_heads / n_kv) / kTileRows + n_req
+                                                                  : static_cast<long long>(n_req) * s.tiles_o);
         places = s.shares > 0 && !s.direct() ? (units + s.shares) * n_kv : 0;
         o = 0;
         ml = o + rows * hd * sizeof(float);

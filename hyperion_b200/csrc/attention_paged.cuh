@@ -77,8 +77,18 @@ struct SharedPlan {
     int prefix_unit = 0;     // 16-row kernel: one tile of all rows against the prefix
     int tiles_o = 0;         // 16-row tiles of one request (0: not launched)
     int o_prefix = 0;        // they cover the prefix too
+    int unit_req = 0, unit_rows = 0;  // how units are numbered, see unit_of
     int one_part = 0;        // a CTA takes a whole unit and writes the output
     int shares = 0;          // otherwise: shares of every KV head's slices, a warp each
+    // The number of a 16-row unit: tile `tile` of request `req`, whose rows start at token t0. By request
+    // (tiles_o numbers each) where all have tiles_o tiles or nearly so. Where one is much longer than the
+    // others (a prefill chunk beside single rows) that would count every request as the longest, so there
+    // t0 * G / 16 + req + tile for G rows a token: a request of n rows begins at a number at least
+    // ceil(n / 16) below the next one's, as floor(x + y) + 1 >= floor(x) + ceil(y), and all stay below
+    // T * G / 16 + n_req.
+    __host__ __device__ int unit_of(int req, int t0, int tile) const {
+        return prefix_unit + tile + req * unit_req + static_cast<int>(static_cast<unsigned long long>(t0) * unit_rows / 16);
+    }
     // nothing has to be joined
     __host__ __device__ bool direct() const { return one_part != 0 || (tc_per_request != 0 && tc_splits == 1); }
 };

@@ -105,6 +105,27 @@ def test_attn_prefix_pages_that_no_row_sees(built_lib, prefix):
     b.check(got)
 
 
+@pytest.mark.parametrize("hd,window,softcap", [(64, 0, 0.0), (128, 0, 20.0), (128, 300, 0.0), (256, 0, 0.0)])
+@pytest.mark.parametrize("prefix,chunk", [(0, 900), (30, 40), (400, 900), (2000, 300), (2000, 40)])
+def test_attn_decode_rows_beside_a_chunk(built_lib, hd, window, softcap, prefix, chunk):
+    """One step of many single rows and one request's long chunk of new rows; the scratch is used within its bounds."""
+    import torch
+    from hyperion_b200 import ops
+    rng = np.random.default_rng(hd)
+    own = rng.integers(1, 200, 40)
+    q = np.ones(40, np.int64)
+    q[:3], q[17], q[39] = [0, 2, 1], chunk, 19
+    own[17], own[0], own[39] = chunk + 50, 30, 20
+    b = Batch(8, 4, hd, 32, prefix, own, q, seed=hd + window, window=window, softcap=softcap, lead=1, pad_rows=3)
+    scratch = ops.SharedPrefixScratch(b.T, 40, chunk, int(own.max()), prefix, 8, 4, hd)
+    whole = torch.full((scratch.nbytes + 4096,), 77, dtype=torch.uint8, device="cuda")
+    scratch.buf = whole[:scratch.nbytes]
+    first = int(b.start[17])
+    rows = list(range(1, first + 3, 3)) + [first + chunk // 2 - 1, first + chunk - 3, first + chunk - 2, first + chunk - 1, first + chunk]
+    b.check(b.call(scratch=scratch), rows=rows + list(range(int(b.start[39]), int(b.start[40]), 6)) + [b.T - 4])
+    assert (whole[scratch.nbytes:] == 77).all()
+
+
 # ------------------------------------------------------------------------------ sampling
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("min_p", [1e-12, 1e-14, 1e-20, 1e-37])

@@ -187,6 +187,13 @@ def _ck_opt(name, t, dtype, shape, dev):
     return None if t is None else _ck(name, t, dtype, shape, dev)
 
 
+def _ck_int(names, bits):
+    """ctypes would cut a count to its lower 32 bits. `bits` is the or of them all: out of range where one is and
+    none is negative, and a negative one is refused by the entry point."""
+    if bits >> 31 not in (0, -1):
+        raise ValueError(f"{names} must be below 2^31")
+
+
 def _device(t):
     dev = t.get_device()
     if dev < 0:
@@ -229,10 +236,12 @@ def paged_plan(cached_lens, new_lens, free_pages, block_table, n_pages: int, pag
                plan: PagedPlan | None = None, stream=None) -> PagedPlan:
     """Block tables (in place) and the row tables of a step from the requests' lengths. The lengths may be
     another plan's total_lens, not those of the `plan` that is written."""
+    _ck_int("n_pages, page_size, max_rows, pos0", n_pages | page_size | max_rows | pos0)
     dev, n = _device(cached_lens), cached_lens.numel()
     if block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("block_table is [n_req, max_blocks], free_pages [n_free]")
     width, n_free = block_table.shape[1], free_pages.shape[0]
+    _ck_int("the lengths of cached_lens, block_table and free_pages", n | width | n_free)
     c, a = _ck("cached_lens", cached_lens, _I32, (n,), dev), _ck("new_lens", new_lens, _I32, (n,), dev)
     f, b = _ck("free_pages", free_pages, _I32, (n_free,), dev), _ck("block_table", block_table, _I32, (n, width), dev)
     ctx = _switch(dev, stream)
@@ -251,6 +260,7 @@ def qkv_post_paged(qkv, n_heads, n_kv, hd, v_from_k, q_norm, k_norm, inv_freq, r
                    q_out=None, stream=None):
     """QK-norm, RoPE at row_pos and the cache write to slot_map of the pools [n_pages, page_size,
     n_kv, hd]; returns q [T, n_heads, hd]. qkv [T, ld] may have padded rows (its stride is used)."""
+    _ck_int("n_heads, n_kv, hd", n_heads | n_kv | hd)
     dev = _device(qkv)
     if qkv.dim() != 2 or qkv.dtype is not _BF16 or qkv.stride(1) != 1:
         raise ValueError("qkv is bf16 [T, columns] with unit column stride")
@@ -261,6 +271,7 @@ def qkv_post_paged(qkv, n_heads, n_kv, hd, v_from_k, q_norm, k_norm, inv_freq, r
     shape = k_pool.shape
     if len(shape) != 4 or shape[2] != n_kv or shape[3] != hd:
         raise ValueError("k_pool is [n_pages, page_size, n_kv, hd]")
+    _ck_int("the rows of qkv, their stride and the slots of the pools", T | ld | shape[0] * shape[1])
     ctx = _switch(dev, stream)
     if ctx is not None:
         with ctx:
@@ -282,6 +293,7 @@ class SharedPrefixScratch:
     larger one serves any call that needs no more bytes."""
 
     def __init__(self, T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd, device="cuda"):
+        _ck_int("T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd", T | n_req | max_q | max_own | prefix_len | n_heads | n_kv | hd)
         n = lib().hyb_sdpa_shared_prefix_scratch_bytes(T, n_req, max_q, max_own, prefix_len, n_heads, n_kv, hd)
         if n == 0:
             raise ValueError("sdpa_shared_prefix: bad shape")
@@ -293,6 +305,7 @@ def sdpa_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len: int, block_t
                        max_own: int, window=0, scale=1.0, softcap=0.0, scratch: SharedPrefixScratch | None = None, out=None,
                        stream=None):
     """Attention of rows q [T, H, hd] over the shared prefix and their requests' own pages."""
+    _ck_int("prefix_len, max_q, max_own, window", prefix_len | max_q | max_own | window)
     dev = _device(q)
     shape = q.shape
     if len(shape) != 3 or k_pool.dim() != 4 or block_table.dim() != 2:
@@ -301,6 +314,7 @@ def sdpa_shared_prefix(q, k_pool, v_pool, prefix_table, prefix_len: int, block_t
     pool = k_pool.shape
     n_pages, page, nkv, _ = pool
     n, width = own_lens.numel(), block_table.shape[1]
+    _ck_int("the sizes of q, the pools and block_table", T | H | n_pages | page | n | width)
     if prefix_len < 0 or (prefix_len > 0 and (prefix_table is None or prefix_table.numel() * page < prefix_len)):
         raise ValueError("prefix_table does not hold prefix_len keys")
     if pool[3] != hd:
@@ -334,6 +348,7 @@ def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     if logits.dim() != 2 or (dtype is not _BF16 and dtype is not _F32) or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits is bf16 or float32 [rows, vocab] with unit column stride")
     n, V = logits.shape
+    _ck_int("the sizes of logits", n | V)
     ld = logits.stride(0) if n > 1 else V
     if ld < V:
         raise ValueError("the rows of logits overlap")

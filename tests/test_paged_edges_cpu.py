@@ -2,8 +2,10 @@
 import ctypes
 
 import pytest
+import torch
 
 import hyperion_b200 as hb
+from hyperion_b200 import ops
 
 AT = {n: 1 << 20 | i << 16 for i, n in enumerate(["cached", "new", "free", "table", "row_start", "row_req", "row_pos", "slot_map",
                                                   "total_lens", "status"])}  # addresses that are never followed
@@ -49,3 +51,43 @@ def test_scratch_bounds_hold_for_uniform_batches(built_lib):
         G = H // nkv
         units = n * -(-q * G // 16)
         assert f(n * q, n, q, 200, 0, H, nkv, hd) <= 4 * (hd + 2) * 16 * nkv * (units + 592 / nkv + 1) + 8 * units + 4096
+
+
+@pytest.mark.parametrize("i,v", [(4, 1 << 32), (5, (1 << 32) + 16), (6, 1 << 31), (7, 1 << 40), (7, -(1 << 32))])
+def test_plan_sizes_are_not_cut_to_32_bits(built_lib, i, v):
+    x = torch.zeros(2, dtype=torch.int32)
+    args = [x, x, x, torch.zeros(2, 2, dtype=torch.int32), 4, 16, 8, 0]
+    args[i] = v
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.paged_plan(*args)
+
+
+@pytest.mark.parametrize("kw", [dict(window=(1 << 32) + 1), dict(window=1 << 32), dict(max_own=1 << 32), dict(max_q=(1 << 33) + 1),
+                                dict(prefix_len=1 << 32)])
+def test_attention_sizes_are_not_cut_to_32_bits(built_lib, kw):
+    i, pool = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 16, 1, 64, dtype=torch.bfloat16)
+    a = dict(q=torch.zeros(2, 2, 64, dtype=torch.bfloat16), k_pool=pool, v_pool=pool, prefix_table=None, prefix_len=0, block_table=i[None],
+             own_lens=i, row_start=i, row_pos=i, max_q=1, max_own=16)
+    a.update(kw)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.sdpa_shared_prefix(**a)
+
+
+def test_scratch_sizes_are_not_cut_to_32_bits(built_lib):
+    good = [4, 2, 2, 100, 100, 4, 2, 64]
+    assert ops.SharedPrefixScratch(*good, device="cpu").nbytes > 0
+    for i in range(8):
+        bad = list(good)
+        bad[i] += 1 << 32
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops.SharedPrefixScratch(*bad, device="cpu")
+        bad[i] = -1
+        with pytest.raises(ValueError):
+            ops.SharedPrefixScratch(*bad, device="cpu")
+
+
+def test_post_sizes_are_not_cut_to_32_bits(built_lib):
+    pool = torch.zeros(2, 16, 1, 64, dtype=torch.bfloat16)
+    for kw in ((1 << 32 | 2, 1, 64), (2, 1 << 32 | 1, 64), (2, 1, 1 << 32 | 64)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops.qkv_post_paged(torch.zeros(2, 256, dtype=torch.bfloat16), *kw, False, None, None, None, None, None, pool, pool)

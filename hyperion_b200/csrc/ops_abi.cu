@@ -567,6 +567,10 @@ HypStatus hyb_sample_batch(const void* logits, int32_t f32, int32_t rows, int32_
         return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sample_batch: bad shape (1..2^20 rows of 1..2^19 logits)");
     if (reinterpret_cast<uintptr_t>(logits) % (f32 ? 4 : 2) != 0)
         return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sample_batch: logits are not aligned to their type");
+    const size_t n = sizeof(int32_t) * rows, row = f32 ? 4 : 2;
+    if (outputs_overlap({{token, n}, {kept, n}, {prob, n}},
+                        {{logits, (static_cast<size_t>(ld) * (rows - 1) + vocab) * row}, {u, n}, {temperature, n}, {top_k, n}, {top_p, n}, {min_p, n}}))
+        return hyb::abi_fail(HYP_STATUS_INVALID_ARGUMENT, "sample_batch: an output overlaps an input or another output");
     return run([&] {
         hyb::SampleBatchParams p;
         p.logits = logits;

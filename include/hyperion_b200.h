@@ -329,7 +329,7 @@ HypStatus hyb_sdpa_shared_prefix(const void* q, const void* k_pool, const void* 
  *   drawn token's share of the kept weight. NaN logits count as -inf; a row without any
  *   logit above -inf gives token -1, kept 0, prob 0; +inf logits share all the weight.
  *   u outside [0, 1) is clamped. Sums are exact integers: results do not depend on the
- *   batch, the order of additions or the run.
+ *   batch, the order of additions or the run. No output may overlap an input or another output.
  */
 HypStatus hyb_sample_batch(const void* logits, int32_t f32, int32_t rows, int32_t vocab, int64_t ld, const float* u,
                            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,

@@ -91,3 +91,14 @@ def test_post_sizes_are_not_cut_to_32_bits(built_lib):
     for kw in ((1 << 32 | 2, 1, 64), (2, 1 << 32 | 1, 64), (2, 1, 1 << 32 | 64)):
         with pytest.raises(ValueError, match="2\\^31"):
             ops.qkv_post_paged(torch.zeros(2, 256, dtype=torch.bfloat16), *kw, False, None, None, None, None, None, pool, pool)
+
+
+@pytest.mark.parametrize("moved,onto,by", [("prob", "u", 0), ("token", "top_k", 0), ("kept", "token", 4), ("prob", "temperature", -8),
+                                           ("u", "kept", 8), ("token", "logits", 1200), ("prob", "min_p", 8), ("kept", "top_p", 0)])
+def test_sample_refuses_overlapping_outputs(built_lib, moved, onto, by):
+    at = {n: 1 << 20 | i << 16 for i, n in enumerate(["logits", "u", "temperature", "top_k", "top_p", "min_p", "token", "kept", "prob"])}
+    at[moved] = at[onto] + by
+    p = {k: ctypes.c_void_p(v) for k, v in at.items()}
+    assert built_lib.hyb_sample_batch(p["logits"], 1, 3, 100, 104, p["u"], p["temperature"], p["top_k"], p["top_p"], p["min_p"], p["token"],
+                                      p["kept"], p["prob"], None) == hb.INVALID_ARGUMENT
+    assert "overlap" in hb.last_error()

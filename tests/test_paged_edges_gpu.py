@@ -126,6 +126,28 @@ def test_attn_decode_rows_beside_a_chunk(built_lib, hd, window, softcap, prefix,
     assert (whole[scratch.nbytes:] == 77).all()
 
 
+@pytest.mark.parametrize("H,nkv,hd,B,prefix,softcap", [(8, 4, 64, 200, 3000, 0.0), (8, 4, 128, 200, 3000, 0.0), (16, 8, 256, 96, 3001, 0.0),
+                                                       (8, 4, 128, 200, 3000, 30.0), (32, 16, 128, 64, 2500, 0.0)])
+def test_attn_window_of_a_large_decode_batch(built_lib, H, nkv, hd, B, prefix, softcap):
+    """Tiles of 128 rows of many requests at different positions, whose windows reach into the prefix or not; the pages
+    in front of every window are gone. All of these go the way of the prefix by whole-batch tiles of the 128-row
+    kernel, the own keys by the 16-row kernel and a merge."""
+    import torch
+    rng = np.random.default_rng(B + hd)
+    own = rng.integers(1, 120, B)
+    own[::7] = rng.integers(1000, 1400, len(own[::7]))  # around the window
+    own[3:6], own[-1] = [1023, 1024, 1025], 1400
+    b = Batch(H, nkv, hd, 16, prefix, own, [1] * B, seed=hd, window=1024, softcap=softcap)
+    tab, table = b.ptab.copy(), b.table.copy()
+    b.ptab[:(prefix - 1024 + 1) // 16] = -1
+    for i in range(B):
+        b.table[i, :max(0, int(own[i]) - 1024) // 16] = 10 ** 6
+    got = b.call()
+    b.ptab, b.table = tab, table
+    assert torch.isfinite(got).all()
+    b.check(got, rows=sorted({0, 3, 4, 5, 7, 63, 64, B - 1} | set(rng.choice(B, 12, replace=False).tolist())))
+
+
 # ------------------------------------------------------------------------------ sampling
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("min_p", [1e-12, 1e-14, 1e-20, 1e-37])

@@ -297,7 +297,9 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   a key may be anything. A negative own_lens counts as 0.
  *   A request's rows are taken to stand at neighbouring positions: slots before the first and
  *   after the last key that its rows see may hold anything (NaN included), those between
- *   must be finite.
+ *   must be finite. Rows of several requests share tiles against the prefix: where some stand
+ *   inside it (row_pos < prefix_len - 1) and a window is set, the same holds for the prefix's slots
+ *   between the first and the last key that any row of the call sees, and for their pages.
  * n_req is 1..1024; head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; n_pages *
  * page_size < 2^31; q, the pools, out and scratch 16-byte aligned, and neither out nor scratch
  * overlaps anything else. A call is refused when its steps of 16 keys, by the bounds and for every

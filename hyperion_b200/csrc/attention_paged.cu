@@ -5,15 +5,19 @@
 // [0, prefix_len) and the request's own keys j < own_len at positions prefix_len + j, both
 // only up to pos and, with a window, after pos - window. With s = scale * q.k (soft-capped
 // when asked) the output is sum_j exp(s_j) v_j / sum_j exp(s_j). A softmax over a set of
-// keys is joined exactly from its parts: a part keeps m = max s, l = sum exp(s - m) and
-// o = sum exp(s - m) v, and the whole is sum_i exp(m_i - M) o_i / sum_i exp(m_i - M) l_i.
+// keys is joined exactly from its parts: a part keeps a reference m, l = sum exp(s - m) and
+// o = sum exp(s - m) v, and the whole is sum_i exp(m_i - M) o_i / sum_i exp(m_i - M) l_i with
+// M = max m_i, whatever the references. m is a maximum that the part met and moves only when the
+// scores outgrow it by a factor of 2^40 (kSharedLazy).
 // So the prefix is one part for the batch (its keys are read once, with the rows of all
 // requests as one matrix), each request's pages are others, long parts are split over the
 // SMs, and shared_merge_kernel joins them.
 //
 // Statistics and accumulators are fp32. The probabilities are rounded to bf16 for the
-// tensor cores, as unnormalised exp(s - m) <= 1, and l sums the rounded ones, so that the
-// rounding cancels where all weights round alike.
+// tensor cores, as unnormalised exp(s - m), and l sums the rounded ones, so that the rounding
+// cancels where all weights round alike. They reach 2^40 and not only 1; bf16 has fp32's
+// exponents, so that costs no precision, and sums over 2^31 keys stay finite for |v| below 2^56.
+// l is at least 1 for a row that sees a key, and the factors exp(m_i - M) are at most 1.
 #include "attention_paged.cuh"
 #include "tma.cuh"
 
@@ -87,7 +91,10 @@ bool only_way(const Sizes& z, Way* way) {
     return true;
 }
 
-// Otherwise by what they take, in microseconds (the constants as measured).
+// Otherwise by what they take, in microseconds. The constants are measured without a soft-cap, for
+// requests of equal rows and about one tile an SM. They count one start for all the tiles that an SM
+// takes in turn, no soft-cap and every request as long as max_q: many requests with short keys, the
+// more so with a soft-cap, and ragged batches can go a slower way than they had to.
 Way way_of(const Sizes& z, int window) {
     Way way;
     if (only_way(z, &way)) return way;
@@ -215,8 +222,8 @@ struct SmallPlan {
 // the bandwidth. ONE: short units, a CTA takes a whole one, joins its four warps and writes
 // the output itself. PLAIN: no soft-cap and a positive scale, so that a row's maximum is that of its
 // raw products.
-// 64 requests of up to 1024 own tokens, 32 query and 16 KV heads of 128: 50 us, 6.4 TB/s in its steady
-// part. ONE, a request of 50 keys: 6.6 us.
+// 64 requests of up to 1024 own tokens, 32 query and 16 KV heads of 128 (269 MB): 54 us behind the prefix
+// kernel, 4.9 TB/s. ONE, a request of 50 keys: 6.7 us, 4 of them the kernel.
 template <int HD, bool ONE, bool PLAIN>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     shared_attn_small_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,

@@ -27,8 +27,8 @@
 // Every mbarrier wait is bounded; TMEM is freed before the CTA exits.
 //
 // Measured on a B200. head_dim 256, 16 query and 8 KV heads, 8 requests of 200 to 300 rows on a
-// prefix of 8192 and up to 600 own tokens: 324 us, 846 TFLOP/s, half of what a large dense
-// product reaches. A 64-key block takes some 2100 cycles, its products alone 1270 of them (a
+// prefix of 8192 and up to 600 own tokens: 324 us, 846 TFLOP/s (332 to 347 us once the clock gives way
+// under load), half of what a large dense product reaches. A 64-key block takes some 2100 cycles, its products alone 1270 of them (a
 // product of 128 x 64 x 16 takes 47, of 128 x 128 x 16 64, of 128 x 256 x 16 128); the rest is the chain
 // softmax(c) -> P V(c) -> S(c + 2) of the two blocks in flight, and the waits and commits of the issuing
 // warp between its products (a wait on a complete barrier 109 cycles, a commit 40). Copies of the

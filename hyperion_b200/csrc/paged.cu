@@ -34,7 +34,7 @@ namespace {
 // integers are latency, not work, so every CTA repeats them over all requests (the lengths
 // come from L2 after the first) instead of paying a second launch, and then fills its share
 // of the rows: row r finds its request by binary search in the row starts, in shared memory.
-// 64 requests of one token: 7.5 us; 512 requests of 1 to 1023 tokens (6.4 MB): 13.2 us.
+// 64 requests of one token: 8.5 us; 512 requests of 1 to 1023 tokens (6.4 MB): 12.6 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 
@@ -210,14 +210,15 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPla
 
 // ------------------------------------------------------------------------------ append
 // y = x * rsqrt(mean(x^2) + eps) * w (v: without w); RoPE turns the pair (e, e + hd/2) of q
-// and k by pos * inv_freq[e]; everything in fp32, rounded to bf16 once. Bound by HBM: each
-// projection row is read once and written once. A group of hd/16 lanes owns one head and
+// and k by pos * inv_freq[e]; everything in fp32, rounded to bf16 once. Each projection row is
+// read once and written once; what bounds it is a row's chain (position, angles in double, a
+// barrier, load, reduction, store) with nothing of the next row in flight. A group of hd/16 lanes owns one head and
 // each lane 8 neighbouring elements of either half (two 16-byte accesses, and both ends of
 // a pair in one lane), so a warp handles 512/hd heads at once; the row's hd/2 sines and
 // cosines are computed once in shared memory for all its heads. Angles are reduced in
 // double: pos * inv_freq in fp32 would be off by 2^-24 * pos radians (0.008 at 131072).
-// 2048 rows of 16 query and 8 KV heads of 256: 15.1 us for 67 MB (4.5 TB/s) with the data in
-// L2, 22 us from HBM; 64 rows of 32 + 16 heads of 128: 5.1 us.
+// 2048 rows of 16 query and 8 KV heads of 256 (67 MB): 22.5 us from HBM (3.0 TB/s; the bytes alone
+// 10.2), 15.0 with the data in L2; 64 rows of 32 + 16 heads of 128: 5.2 us.
 constexpr int kPostThreads = 256;
 
 template <int HD>

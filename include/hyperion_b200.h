@@ -286,7 +286,7 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   b's own key j < own_lens[b] (block_table [n_req, max_blocks]) at prefix_len + j. Row t
  *   sees the keys at positions <= row_pos[t] and, with window > 0, > row_pos[t] - window.
  *   scale and softcap as in hyb_sdpa_decode; scores, statistics and sums are fp32, the
- *   unnormalised probabilities are rounded to bf16.
+ *   unnormalised probabilities are rounded to bf16. They reach 2^40: values are below 2^56.
  *   A row that sees no key gets zeros. Rows of no request (before row_start[0] or from
  *   row_start[n_req] on) and rows with row_pos < 0 stay as they were.
  *   max_q and max_own are host bounds on a request's rows and own keys: they size the launch

@@ -42,7 +42,7 @@ struct Span {
     size_t bytes;
     bool meets(const Span& o) const {
         const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
-        return p && o.p && a < b + o.bytes && b < a + bytes;
+        return p && o.p && bytes && o.bytes && a < b + o.bytes && b < a + bytes;
     }
 };
 bool outputs_overlap(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {

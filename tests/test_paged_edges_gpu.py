@@ -61,6 +61,17 @@ def test_plan_stepped_from_its_own_lengths(built_lib):
             ops.paged_plan(lens, torch.ones(n, dtype=torch.int32, device="cuda"), free, table, 4000, page, rows, plan=plan)
 
 
+def test_plan_empty_free_list_overlaps_nothing(built_lib):
+    import torch
+    import hyperion_b200 as hb
+    from hyperion_b200 import ops
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    cached, new, table, plan = i32(3, 5), i32(1, 2), i32(4, 7), ops.PagedPlan(2, 4)
+    hb.check(built_lib.hyb_paged_plan(cached.data_ptr(), new.data_ptr(), 2, 16, 8, plan.slot_map.data_ptr() + 4, 0, table.data_ptr(), 1, 0, 4,
+                                      *plan._at, torch.cuda.current_stream().cuda_stream))
+    assert plan.slot_map.tolist() == [4 * 16 + 3, 7 * 16 + 5, 7 * 16 + 6, -1] and plan.status.tolist() == [0, 3, 0, 0]
+
+
 # ----------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("B,q,prefix", [(2, 150, 300), (2, 1, 30), (40, 1, 300), (4, 1, 300)])

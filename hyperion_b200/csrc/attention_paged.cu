@@ -192,6 +192,13 @@ __device__ __forceinline__ Request request_of(const SharedAttnParams& p, int req
     return r;
 }
 
+// The position of row t of that request (-1: of all rows, of which those of no request see nothing,
+// whatever their positions say: they would widen the window of the others' tile).
+__device__ __forceinline__ int pos_of(const SharedAttnParams& p, int req, int t) {
+    const int pos = p.row_pos[t];
+    return req < 0 && (t < p.row_start[0] || t >= p.row_start[p.n_req]) ? -1 : pos;
+}
+
 template <int HD>
 struct SmallPlan {
     // K or V of one slice is one stage, head_dim / 64 boxes of [16 keys][128 bytes]; 24 KB a warp,
@@ -250,11 +257,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     const int my_warp = blockIdx.x * kWarps + warp, my_share = my_warp / p.n_kv, my_hk = my_warp % p.n_kv;
     if constexpr (!ONE) {
         // positions matter for the number of slices only where a window cuts the keys
-        auto span = [&](const Request& r, int& lo, int& hi) {
+        auto span = [&](int req, const Request& r, int& lo, int& hi) {
             lo = INT_MAX;
             hi = -1;
             for (int t = 0; p.window > 0 && t < r.n_tok; ++t) {
-                const int pos = p.row_pos[r.t0 + t];
+                const int pos = pos_of(p, req, r.t0 + t);
                 if (pos >= 0) {
                     lo = min(lo, pos);
                     hi = max(hi, pos);
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         };
         int lo, hi;
         if (pl.prefix_unit) {
-            span(request_of(p, -1), lo, hi);
+            span(-1, request_of(p, -1), lo, hi);
             prefix_slices = keys_of(nullptr, 0, p.prefix_len, lo, hi, p.window).slices;
         }
         const int per = (p.n_req + kWarps * 32 - 1) / (kWarps * 32);
@@ -271,7 +278,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         unsigned sum = 0;
         for (int b = b0; b < b1 && pl.tiles_o > 0; ++b) {
             const Request r = request_of(p, b);
-            span(r, lo, hi);
+            span(b, r, lo, hi);
             const int n = keys_of(nullptr, p.prefix_len, r.own, lo, hi, p.window).slices +
                           (pl.o_prefix ? keys_of(nullptr, 0, p.prefix_len, lo, hi, p.window).slices : 0);
             s_slices[b] = n;
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (ONE && rows <= 0) return;
     // lane m (and m + 16): row m's position and place
     const int mm = m0 + min(lane & 15, rows - 1), tok = mm / G;
-    const int my_pos = (lane & 15) < rows ? p.row_pos[t0 + tok] : -1;
+    const int my_pos = (lane & 15) < rows ? pos_of(p, req, t0 + tok) : -1;
     const int my_row = (t0 + tok) * p.n_heads + hk * G + (mm - tok * G);
     const int g = lane >> 2, c2 = 2 * (lane & 3);
     uint32_t qf[KS][4];
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     int pmin = my_pos < 0 ? INT_MAX : my_pos, pmax = my_pos;
     if (!ONE && p.window > 0)
         for (int t = lane; t < rq.n_tok; t += 32) {
-            const int pos = p.row_pos[t0 + t];
+            const int pos = pos_of(p, req, t0 + t);
             if (pos >= 0) pmin = min(pmin, pos);
             pmax = max(pmax, pos);
         }

@@ -179,9 +179,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     id /= p.n_kv;
     const bool per_request = pl.tc_per_request != 0;
     const int tile = per_request ? id % pl.tc_tiles : id, req = per_request ? id / pl.tc_tiles : 0;
-    int t0 = 0, n_tok = p.T, own = 0;
+    int t0 = 0, n_tok = p.T, own = 0, begin = 0, end = INT_MAX;
     bool broken = false;
-    if (per_request) {
+    if (!per_request) {
+        // rows of no request see nothing, whatever their positions say: they would widen the window of the others
+        begin = p.row_start[0];
+        end = p.row_start[p.n_req];
+    } else {
         const int first = p.row_start[req], next = p.row_start[req + 1], len = p.own_lens[req];
         const long long most = min(static_cast<long long>(p.max_own), static_cast<long long>(p.max_blocks) * p.page_size);
         t0 = min(max(first, 0), p.T);
@@ -241,7 +245,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < kSoftWarps) {
         const int pr = static_cast<int>(m0) + min(r, rows - 1), tok = pr / G;
         row = (t0 + tok) * p.n_heads + hk * G + (pr - tok * G);
-        if (r < rows) pos = p.row_pos[t0 + tok];
+        if (r < rows) {
+            pos = p.row_pos[t0 + tok];
+            if (t0 + tok < begin || t0 + tok >= end) pos = -1;
+        }
         const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<size_t>(row) * HD);
 #pragma unroll
         for (int j = 0; j < kQ; ++j)

@@ -288,7 +288,7 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   scale and softcap as in hyb_sdpa_decode; scores, statistics and sums are fp32, the
  *   unnormalised probabilities are rounded to bf16. They reach 2^40: values are below 2^56.
  *   A row that sees no key gets zeros. Rows of no request (before row_start[0] or from
- *   row_start[n_req] on) and rows with row_pos < 0 stay as they were.
+ *   row_start[n_req] on; their positions do not matter) and rows with row_pos < 0 stay as they were.
  *   max_q and max_own are host bounds on a request's rows and own keys: they size the launch
  *   and the scratch (hyb_sdpa_shared_prefix_scratch_bytes with the same values; contents do
  *   not matter before or after). Rows at or past max_q of a request, and rows of a request
@@ -299,7 +299,7 @@ HypStatus hyb_qkv_post_paged(const void* qkv, int32_t T, int32_t ld, int32_t n_h
  *   after the last key that its rows see may hold anything (NaN included), those between
  *   must be finite. Rows of several requests share tiles against the prefix: where some stand
  *   inside it (row_pos < prefix_len - 1) and a window is set, the same holds for the prefix's slots
- *   between the first and the last key that any row of the call sees, and for their pages.
+ *   between the first and the last key that any request's row sees, and for their pages.
  * n_req is 1..1024; head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; n_pages *
  * page_size < 2^31; q, the pools, out and scratch 16-byte aligned, and neither out nor scratch
  * overlaps anything else. A call is refused when its steps of 16 keys, by the bounds and for every

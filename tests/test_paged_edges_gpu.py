@@ -159,6 +159,27 @@ def test_attn_window_of_a_large_decode_batch(built_lib, H, nkv, hd, B, prefix, s
     b.check(got, rows=sorted({0, 3, 4, 5, 7, 63, 64, B - 1} | set(rng.choice(B, 12, replace=False).tolist())))
 
 
+@pytest.mark.parametrize("H,nkv,hd,B,prefix", [(4, 2, 64, 2, 600), (4, 2, 256, 3, 600), (8, 4, 64, 200, 3000), (32, 16, 128, 64, 2500)])
+def test_attn_rows_of_no_request_widen_no_window(built_lib, H, nkv, hd, B, prefix):
+    """Rows before the first and behind the last request, with stale positions, share the tiles of the others: what
+    they would see of the prefix is not looked at."""
+    import torch
+    own = np.random.default_rng(B).integers(1, 40, B)
+    own[-1] = min(1400, 7 * B)
+    window = 50 if B < 10 else 1024
+    b = Batch(H, nkv, hd, 16, prefix, own, [1] * B, seed=hd, window=window, lead=1, pad_rows=2)
+    assert (b.pos[[0, -2, -1]] == 5).all()
+    tab = b.ptab.copy()
+    for page in (None, -1):  # NaN in the slots, then pages that are gone, in front of every window
+        if page is not None:
+            b.ptab[:(prefix - window + 1) // 16] = page
+        got = b.call()
+        saved, b.ptab = b.ptab, tab
+        b.check(got, rows=sorted({1, 2, B // 2, B}))
+        assert torch.isfinite(got).all() and (got[[0, -2, -1]] == 7.0).all()
+        b.ptab = saved
+
+
 # ------------------------------------------------------------------------------ sampling
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("min_p", [1e-12, 1e-14, 1e-20, 1e-37])
